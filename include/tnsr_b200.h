@@ -770,6 +770,157 @@ TNSR_B200_API int tnsr_b200_sample_top_k(const float* logits, uint32_t* out, uin
 TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t rows, uint32_t vocab,
                                    void* stream);
 
+/* ---- beam search over caches in pages --------------------------------------------- */
+/* No reference counterpart: tnsr's decode loop is greedy and its caches are one
+ * slab per session.  A decode step of a beam search is
+ *     beam_select      candidates of a group from its beams' logits: tokens, parents
+ *     pages_fork       sequences take over their parents' pages (reorder_states:
+ *                      recurrent states, contiguous caches)
+ *     pages_reserve    room for the next row; pages that others hold too are copied
+ *     per layer: paged_append (new keys and values), paged_attention
+ * All of it is device work on the caller's stream, without synchronisation.  The
+ * entry points below share these rules.
+ *  - A status word (`d_status`, a device int that the caller clears, may be NULL)
+ *    keeps the first problem that a kernel meets: 3 = a sequence has more rows than
+ *    its table row can name, or fewer than a call brings or needs; 4 = a table
+ *    entry that a call follows names no page of the pool; 5 = more pages wanted than
+ *    are free; 6 = a parent outside its group.  Nothing outside the given tables,
+ *    pools and rows is read or written in such a case.
+ *  - A workspace is device memory, 16-byte aligned, zeroed once before its first
+ *    use (again if a launch was cut short by a device error); calls leave it ready
+ *    for the next one.  Calls that may overlap on the GPU must not share one, and
+ *    two captured graphs that share one must not run at the same time.
+ *  - Descriptions are read before a call returns; host arrays of pointers and sizes
+ *    too. */
+
+/* The `keep` best of a group's beams x vocabulary candidates, best first.
+ *     score(b, t) = scores[b] + (logits[b, t] - log sum_j exp logits[b, j])
+ * in f64.  Of equal scores the earlier beam comes first, of a beam's equal logits
+ * the smaller token.  A finished beam has one candidate, end_token with scores[b]
+ * as it is; its other tokens count as -inf, and so do all tokens of a beam whose
+ * score is not finite or whose logits hold NaN, +inf or nothing but -inf (such
+ * tokens fill up what better ones leave, by beam and token).  logits
+ * [groups * beams, logits_ld] of type dtype; scores, finished [groups * beams];
+ * next_scores, tokens, parents, next_finished [groups, keep], none of which may
+ * overlap an input.  parents are rows of `logits` (group * beams + beam).
+ * next_finished: the parent was finished or the token is end_token (0xffffffff: no
+ * such token).  1 <= beams <= 32, 1 <= keep <= 64, keep <= beams * vocab, vocab <= 2^26. */
+typedef struct tnsr_b200_beam_select_args {
+    const void* logits;
+    const float* scores;
+    const uint8_t* finished;      /* NULL: none is */
+    float* next_scores;
+    uint32_t *tokens, *parents;
+    uint8_t* next_finished;       /* may be NULL */
+    void* workspace;              /* tnsr_b200_beam_select_workspace(); its contents do not matter */
+    uint64_t workspace_bytes, logits_ld;
+    uint32_t groups, beams, vocab, keep, end_token;
+    int32_t dtype;
+} tnsr_b200_beam_select_args;
+TNSR_B200_API uint64_t tnsr_b200_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep);
+TNSR_B200_API int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, void* stream);
+
+/* Row i of every tensor becomes what row parents[i] was, in place; parents[i] lies
+ * in i's group (rows group * beams .. group * beams + beams - 1; beams <= 32), else row i stays and the status word says
+ * 6.  Tensor t: rows of row_bytes[t] bytes, pitches[t] bytes apart (so that of a
+ * contiguous cache [sequences, capacity, width] the live prefix alone can move).
+ * parents: device memory, as beam_select wrote them. */
+TNSR_B200_API int tnsr_b200_reorder_states(void* const* tensors, const uint64_t* row_bytes, const uint64_t* pitches, uint32_t count,
+                                           const uint32_t* parents, uint32_t groups, uint32_t beams, int* d_status, void* stream);
+
+/* Who holds which page of a pool.  table [sequences, table_ld]: the pages of a
+ * sequence in order, the first ceil(lengths / page_rows) entries of a row live, the
+ * others never read.  holders [pool_pages]: live entries that name the page, 0 for a
+ * free one.  An empty book is lengths and holders of zero.  sequences <= 12288. */
+typedef struct tnsr_b200_page_book {
+    uint32_t *table, *lengths, *holders;
+    void* workspace;              /* tnsr_b200_pages_workspace() bytes */
+    int* d_status;
+    uint64_t workspace_bytes;
+    uint32_t sequences, table_ld, page_rows, pool_pages;
+} tnsr_b200_page_book;
+/* The pools that a book speaks of (keys and values of every layer): page i of pool t
+ * is page_bytes[t] bytes at tensors[t] + i * page_bytes[t].  `tensors` and
+ * `page_bytes` are host arrays. */
+typedef struct tnsr_b200_page_pools {
+    void* const* tensors;
+    const uint64_t* page_bytes;
+    uint32_t count, pad0;
+} tnsr_b200_page_pools;
+TNSR_B200_API uint64_t tnsr_b200_pages_workspace(uint32_t sequences, uint32_t pool_pages);
+/* Sequence i becomes what sequence parents[i] was (any sequence; itself: it stays):
+ * its pages, held once more, and its length.  No page is copied. */
+TNSR_B200_API int tnsr_b200_pages_fork(const tnsr_b200_page_book* book, const uint32_t* parents, void* stream);
+/* Room for rows[s] more rows (device array; NULL: rows_each for every sequence) of
+ * every sequence, and lengths raised by them.  Free pages are handed out lowest
+ * first, in order of the sequences.  A part-filled last page that other entries
+ * hold too is replaced by a copy in all pools, for every sequence that gets rows
+ * but the first one of them if nobody else holds the page.  If the free pages do
+ * not suffice (5), or a sequence would outgrow its table row (3), or a last page's
+ * entry is not one (4), the status word says so and nothing has changed. */
+TNSR_B200_API int tnsr_b200_pages_reserve(const tnsr_b200_page_book* book, const tnsr_b200_page_pools* pools, const uint32_t* rows,
+                                          uint32_t rows_each, void* stream);
+/* Sequences s with gone[s] != 0 (device bytes) give their pages back and have length 0. */
+TNSR_B200_API int tnsr_b200_pages_release(const tnsr_b200_page_book* book, const uint8_t* gone, void* stream);
+/* Moves the live pages behind the first n (n: how many pages are live) into the free
+ * pages among the first n, in order, in all pools, so that pages n and later are
+ * free.  *live_pages (device, may be NULL) receives n. */
+TNSR_B200_API int tnsr_b200_pages_compact(const tnsr_b200_page_book* book, const tnsr_b200_page_pools* pools, uint32_t* live_pages, void* stream);
+/* Page from[i] onto page to[i] of every pool (device arrays of `pairs` pages); no page
+ * may be the target of two pairs, nor target of one and source of another.  Pairs
+ * outside the pool are left out (status 4). */
+TNSR_B200_API int tnsr_b200_pages_copy(const tnsr_b200_page_pools* pools, const uint32_t* from, const uint32_t* to, uint32_t pairs,
+                                       uint32_t pool_pages, int* d_status, void* stream);
+
+/* New rows of keys and values into their pages.  Sequence s brings rows
+ * row_starts[s] .. row_starts[s + 1] (device [sequences + 1], in order, at most
+ * `chunk` each) or, with row_starts NULL, `chunk` rows each; they are the last rows
+ * of its lengths[s].  rows: how many the arrays hold; rows of no sequence are left
+ * out.  k [rows, kv_heads, dim] with k_ld elements between rows, v likewise with
+ * vdim: slices of a fused projection will do.  Element (page, row, head, i) of a
+ * pool lies at page * k_page + row * k_row + head * k_head + i, in elements; three
+ * zeros stand for [pool_pages, page_rows, kv_heads, dim].  Pages that others hold are
+ * the business of pages_reserve. */
+typedef struct tnsr_b200_paged_append_args {
+    const void *k, *v;
+    void *k_pool, *v_pool;
+    const uint32_t *table, *lengths, *row_starts;
+    int* d_status;
+    uint64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    uint32_t sequences, chunk, rows, k_ld, v_ld, kv_heads, dim, vdim, table_ld, page_rows, pool_pages;
+    int32_t dtype;
+} tnsr_b200_paged_append_args;
+TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args, void* stream);
+
+/* Grouped-query attention of a sequence's newest rows over its cache in pages, which
+ * holds their own keys already: out[row, h] = softmax_j(scale q . k_j) . v_j over the
+ * keys that the row sees.  Rows, strides and lengths as for paged_append: row i of n
+ * is at position p = lengths[s] - n + i and sees j <= p; with window > 0 those with
+ * j > p - window and, beside them, j < sinks.  Pages that no row sees are not
+ * looked at.  A row that sees nothing (lengths[s] < n) gives zeros; rows of no
+ * sequence are left as they were.  q [rows, heads, dim] with q_ld and out
+ * [rows, heads, vdim] with out_ld elements between rows; head h reads key/value
+ * head h / (heads / kv_heads).  dim, vdim <= 256.  Scores, maxima, sums and
+ * accumulators are f32; with dtype bf16 the weights of a value product keep 16
+ * bits for few rows, 8 bits for many.  Keys in a page outside the pool (status 4)
+ * count as zeros.  Status 2: a bounded wait inside the kernel for many rows gave up.
+ * workspace: tnsr_b200_paged_attention_workspace() bytes; NULL: the keys of a
+ * sequence are not divided. */
+typedef struct tnsr_b200_paged_attention_args {
+    const void *q, *k_pool, *v_pool;
+    const uint32_t *table, *lengths, *row_starts;
+    void* out;
+    void* workspace;
+    int* d_status;
+    uint64_t workspace_bytes;
+    uint64_t k_page, k_row, k_head, v_page, v_row, v_head;
+    uint32_t sequences, chunk, rows, q_ld, out_ld, heads, kv_heads, dim, vdim, table_ld, page_rows, pool_pages, window, sinks;
+    float scale;
+    int32_t dtype;
+} tnsr_b200_paged_attention_args;
+TNSR_B200_API uint64_t tnsr_b200_paged_attention_workspace(uint32_t dim, uint32_t vdim, int dtype);
+TNSR_B200_API int tnsr_b200_paged_attention(const tnsr_b200_paged_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

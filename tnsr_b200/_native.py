@@ -101,6 +101,35 @@ class Mamba2Args(C.Structure):
         [("eps", C.c_float), ("dtype", C.c_int32), ("engine", C.c_int32), ("pad0", C.c_uint32)]
 
 
+class BeamSelectArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "scores", "finished", "next_scores", "tokens", "parents", "next_finished", "workspace")] + \
+        [(n, C.c_uint64) for n in ("workspace_bytes", "logits_ld")] + \
+        [(n, C.c_uint32) for n in ("groups", "beams", "vocab", "keep", "end_token")] + [("dtype", C.c_int32)]
+
+
+class PageBook(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("table", "lengths", "holders", "workspace", "d_status")] + [("workspace_bytes", C.c_uint64)] + \
+        [(n, C.c_uint32) for n in ("sequences", "table_ld", "page_rows", "pool_pages")]
+
+
+class PagePools(C.Structure):
+    _fields_ = [("tensors", C.POINTER(C.c_void_p)), ("page_bytes", C.POINTER(C.c_uint64)), ("count", C.c_uint32), ("pad0", C.c_uint32)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_pool", "v_pool", "table", "lengths", "row_starts", "d_status")] + \
+        [(n, C.c_uint64) for n in ("k_page", "k_row", "k_head", "v_page", "v_row", "v_head")] + \
+        [(n, C.c_uint32) for n in ("sequences", "chunk", "rows", "k_ld", "v_ld", "kv_heads", "dim", "vdim", "table_ld", "page_rows", "pool_pages")] + \
+        [("dtype", C.c_int32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_pool", "v_pool", "table", "lengths", "row_starts", "out", "workspace", "d_status")] + \
+        [(n, C.c_uint64) for n in ("workspace_bytes", "k_page", "k_row", "k_head", "v_page", "v_row", "v_head")] + \
+        [(n, C.c_uint32) for n in ("sequences", "chunk", "rows", "q_ld", "out_ld", "heads", "kv_heads", "dim", "vdim", "table_ld", "page_rows", "pool_pages",
+                                   "window", "sinks")] + [("scale", C.c_float), ("dtype", C.c_int32)]
+
+
 _vp, _u32, _u64, _i, _f = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float
 _fp, _u32p = C.POINTER(C.c_float), C.POINTER(C.c_uint32)
 
@@ -167,6 +196,18 @@ SIGNATURES = {
     "tnsr_b200_experts_workspace": (_u64, [_u32, _u32, _u32, _u32, _u32, _i]),
     "tnsr_b200_experts": (_i, [C.POINTER(ExpertsArgs), _vp]),
     "tnsr_b200_sample_top_k": (_i, [_vp, _vp, _u32, _u32, _f, _u32, _u64, _u32, _u32, _vp]),
+    "tnsr_b200_beam_select_workspace": (_u64, [_u32, _u32, _u32, _u32]),
+    "tnsr_b200_beam_select": (_i, [C.POINTER(BeamSelectArgs), _vp]),
+    "tnsr_b200_reorder_states": (_i, [C.POINTER(_vp), C.POINTER(_u64), C.POINTER(_u64), _u32, _vp, _u32, _u32, _vp, _vp]),
+    "tnsr_b200_pages_workspace": (_u64, [_u32, _u32]),
+    "tnsr_b200_pages_fork": (_i, [C.POINTER(PageBook), _vp, _vp]),
+    "tnsr_b200_pages_reserve": (_i, [C.POINTER(PageBook), C.POINTER(PagePools), _vp, _u32, _vp]),
+    "tnsr_b200_pages_release": (_i, [C.POINTER(PageBook), _vp, _vp]),
+    "tnsr_b200_pages_compact": (_i, [C.POINTER(PageBook), C.POINTER(PagePools), _vp, _vp]),
+    "tnsr_b200_pages_copy": (_i, [C.POINTER(PagePools), _vp, _vp, _u32, _u32, _vp, _vp]),
+    "tnsr_b200_paged_append": (_i, [C.POINTER(PagedAppendArgs), _vp]),
+    "tnsr_b200_paged_attention_workspace": (_u64, [_u32, _u32, _i]),
+    "tnsr_b200_paged_attention": (_i, [C.POINTER(PagedAttentionArgs), _vp]),
     "tnsr_b200_decoder_set_sampler": (_i, [_vp, _f, _u32, _u64]),
     "tnsr_b200_decoder_release": (_i, [_vp, _u32]),
     "tnsr_b200_decoder_free_pages": (_u32, [_vp]),

@@ -1,9 +1,14 @@
 // extern "C" wrappers of the individual kernels (operator-level entry points of
 // include/tnsr_b200.h).  They queue work on the caller's stream and never
 // synchronise or allocate.
+#include <cmath>
+
+#include "beam.cuh"
 #include "common.cuh"
 #include "feed_forward.cuh"
 #include "mixers.cuh"
+#include "paged.cuh"
+#include "pages.cuh"
 
 using namespace tb;
 
@@ -28,6 +33,31 @@ struct OverlapLaunches {
     }
     ~OverlapLaunches() { t_pdl = before; }
 };
+
+bool two_types(int32_t dtype) { return dtype == TNSR_B200_F32 || dtype == TNSR_B200_BF16; }
+
+// Rows, widths and strides that paged_append and paged_attention share; strides of zero become those of [pages, page_rows, kv_heads, width].
+template <typename Args>
+const char* paged_problem(const Args* args, Args& a) {
+    if (!args || !args->k_pool || !args->v_pool || !args->table || !args->lengths) return "null pointer";
+    a = *args;
+    if (!two_types(a.dtype)) return "dtype must be f32 or bf16";
+    if (a.chunk == 0 || a.kv_heads == 0 || a.dim == 0 || a.vdim == 0 || a.table_ld == 0 || a.page_rows == 0 || a.pool_pages == 0 ||
+        a.page_rows > PAGED_MAX_KEYS)
+        return "sizes must be positive";
+    if (!a.row_starts && (uint64_t)a.sequences * a.chunk != a.rows) return "rows must be sequences * chunk without row_starts";
+    if (a.rows > 0x7fffffffu) return "too many rows";
+    auto fill = [&](uint64_t& page, uint64_t& row, uint64_t& head, uint32_t width) {
+        if (page == 0 && row == 0 && head == 0) {
+            head = width;
+            row = (uint64_t)a.kv_heads * width;
+            page = row * a.page_rows;
+        }
+    };
+    fill(a.k_page, a.k_row, a.k_head, a.dim);
+    fill(a.v_page, a.v_row, a.v_head, a.vdim);
+    return nullptr;
+}
 }  // namespace
 
 extern "C" {
@@ -239,8 +269,6 @@ int tnsr_b200_mamba2(const tnsr_b200_mamba2_args* args, const tnsr_b200_place* p
     return launch_mamba2(m, step_place(place), args->dtype, as_stream(stream));
 }
 
-static bool two_types(int32_t dtype) { return dtype == TNSR_B200_F32 || dtype == TNSR_B200_BF16; }
-
 int tnsr_b200_rotary(const tnsr_b200_rotary_args* args, const tnsr_b200_place* place, void* stream) {
     if (!args || !place || !args->proj || !args->q || !args->k_cache || !args->v_cache || (args->rotary_dims && !args->rotation)) return bad("rotary: null pointer");
     if (!two_types(args->dtype) || args->rotary_layout > TNSR_B200_ROTARY_HALVES) return bad("rotary: bad dtype or layout");
@@ -319,6 +347,139 @@ int tnsr_b200_experts(const tnsr_b200_experts_args* args, void* stream) {
     e.router_scale = args->router_scale; e.norm_offset = args->norm_offset; e.eps = args->eps; e.engine = args->engine;
     int rc = launch_experts(e, args->dtype, as_stream(stream));
     return rc ? rc : launch_experts_combine(e, args->dtype, as_stream(stream));
+}
+
+// ---- beam search over caches in pages ----
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+uint64_t tnsr_b200_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep) {
+    return beam_select_workspace_bytes(groups, beams, vocab, keep);
+}
+
+int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, void* stream) {
+    if (!args || !args->logits || !args->scores || !args->next_scores || !args->tokens || !args->parents || !args->workspace)
+        return bad("beam_select: null pointer");
+    if (!two_types(args->dtype)) return bad("beam_select: dtype must be f32 or bf16");
+    if (args->beams == 0 || args->beams > BEAM_MAX || args->keep == 0 || args->keep > BEAM_MAX_KEEP || args->vocab == 0 || args->vocab > BEAM_MAX_VOCAB ||
+        args->keep > (uint64_t)args->beams * args->vocab || args->logits_ld < args->vocab || (uint64_t)args->groups * args->beams > 0x7fffffffu)
+        return bad("beam_select: 1 to 32 beams, 1 to 64 candidates (no more than there are), a vocabulary of 1 to 2^26 that fits its rows");
+    if (args->workspace_bytes < beam_select_workspace_bytes(args->groups, args->beams, args->vocab, args->keep) || !aligned16(args->workspace))
+        return bad("beam_select: workspace smaller than tnsr_b200_beam_select_workspace() asks for, or not 16-byte aligned");
+    BeamSelect b;
+    b.logits = args->logits; b.scores = args->scores; b.finished = args->finished; b.next_scores = args->next_scores; b.tokens = args->tokens;
+    b.parents = args->parents; b.next_finished = args->next_finished; b.workspace = args->workspace; b.workspace_bytes = args->workspace_bytes;
+    b.logits_ld = args->logits_ld; b.groups = args->groups; b.beams = args->beams; b.vocab = args->vocab; b.keep = args->keep; b.end_token = args->end_token;
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_beam_select(b, args->dtype, as_stream(stream));
+}
+
+int tnsr_b200_reorder_states(void* const* tensors, const uint64_t* row_bytes, const uint64_t* pitches, uint32_t count, const uint32_t* parents,
+                             uint32_t groups, uint32_t beams, int* d_status, void* stream) {
+    if (!parents || (count && (!tensors || !row_bytes || !pitches))) return bad("reorder_states: null pointer");
+    if (beams == 0 || beams > REORDER_MAX_BEAMS || (uint64_t)groups * beams > 0xffffffffu) return bad("reorder_states: 1 to 32 rows in a group");
+    for (uint32_t t = 0; t < count; ++t)
+        if (!tensors[t] || pitches[t] < row_bytes[t] || row_bytes[t] > 0x7fffffffull * 128) return bad("reorder_states: null tensor, or rows that overlap");
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_reorder_states(tensors, row_bytes, pitches, count, parents, groups, beams, d_status, as_stream(stream));
+}
+
+uint64_t tnsr_b200_pages_workspace(uint32_t sequences, uint32_t pool_pages) { return pages_workspace_bytes(sequences, pool_pages); }
+
+static const char* book_problem(const tnsr_b200_page_book* book, bool workspace) {
+    if (!book || !book->table || !book->lengths || !book->holders || (workspace && !book->workspace)) return "null pointer in the book of pages";
+    if (book->table_ld == 0 || book->page_rows == 0 || book->pool_pages == 0 || book->pool_pages > 0x3fffffffu) return "sizes of the book must be positive";
+    if (book->sequences > PAGES_MAX_SEQUENCES) return "a book of pages has at most 12288 sequences";
+    if (workspace && (book->workspace_bytes < pages_workspace_bytes(book->sequences, book->pool_pages) || !aligned16(book->workspace)))
+        return "workspace smaller than tnsr_b200_pages_workspace() asks for, or not 16-byte aligned";
+    return nullptr;
+}
+static const char* pools_problem(const tnsr_b200_page_pools* pools) {
+    if (!pools || (pools->count && (!pools->tensors || !pools->page_bytes))) return "null pointer in the pools";
+    for (uint32_t t = 0; t < pools->count; ++t)
+        if (!pools->tensors[t] || pools->page_bytes[t] == 0 || pools->page_bytes[t] > 0xffffffffu) return "a pool without memory or with pages of no size";
+    return nullptr;
+}
+static PageBook page_book(const tnsr_b200_page_book* b) {
+    return PageBook{b->table, b->lengths, b->holders, b->d_status, b->sequences, b->table_ld, b->page_rows, b->pool_pages, b->workspace};
+}
+static PagePools page_pools(const tnsr_b200_page_pools* p) { return PagePools{p->tensors, p->page_bytes, p->count}; }
+static int bad_pages(const char* what, const char* problem) { return bad((std::string(what) + ": " + problem).c_str()); }
+
+int tnsr_b200_pages_fork(const tnsr_b200_page_book* book, const uint32_t* parents, void* stream) {
+    if (const char* problem = book_problem(book, true)) return bad_pages("pages_fork", problem);
+    if (!parents) return bad("pages_fork: null pointer");
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_pages_fork(page_book(book), parents, as_stream(stream));
+}
+
+int tnsr_b200_pages_reserve(const tnsr_b200_page_book* book, const tnsr_b200_page_pools* pools, const uint32_t* rows, uint32_t rows_each, void* stream) {
+    if (const char* problem = book_problem(book, true)) return bad_pages("pages_reserve", problem);
+    if (const char* problem = pools_problem(pools)) return bad_pages("pages_reserve", problem);
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_pages_reserve(page_book(book), page_pools(pools), rows, rows_each, as_stream(stream));
+}
+
+int tnsr_b200_pages_release(const tnsr_b200_page_book* book, const uint8_t* gone, void* stream) {
+    if (const char* problem = book_problem(book, false)) return bad_pages("pages_release", problem);
+    if (!gone) return bad("pages_release: null pointer");
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_pages_release(page_book(book), gone, as_stream(stream));
+}
+
+int tnsr_b200_pages_compact(const tnsr_b200_page_book* book, const tnsr_b200_page_pools* pools, uint32_t* live_pages, void* stream) {
+    if (const char* problem = book_problem(book, true)) return bad_pages("pages_compact", problem);
+    if (const char* problem = pools_problem(pools)) return bad_pages("pages_compact", problem);
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_pages_compact(page_book(book), page_pools(pools), live_pages, as_stream(stream));
+}
+
+int tnsr_b200_pages_copy(const tnsr_b200_page_pools* pools, const uint32_t* from, const uint32_t* to, uint32_t pairs, uint32_t pool_pages, int* d_status,
+                         void* stream) {
+    if (const char* problem = pools_problem(pools)) return bad_pages("pages_copy", problem);
+    if (pairs && (!from || !to)) return bad("pages_copy: null pointer");
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_pages_copy(page_pools(pools), from, to, pairs, pool_pages, d_status, as_stream(stream));
+}
+
+int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args, void* stream) {
+    tnsr_b200_paged_append_args a;
+    if (const char* problem = paged_problem(args, a)) return bad_pages("paged_append", problem);
+    if (!a.k || !a.v) return bad("paged_append: null pointer");
+    if (a.k_ld < (uint64_t)a.kv_heads * a.dim || a.v_ld < (uint64_t)a.kv_heads * a.vdim) return bad("paged_append: rows must hold every head");
+    PagedAppend p;
+    p.k = a.k; p.v = a.v; p.k_pool = a.k_pool; p.v_pool = a.v_pool; p.table = a.table; p.lengths = a.lengths; p.row_starts = a.row_starts;
+    p.d_status = a.d_status; p.k_page = a.k_page; p.k_row = a.k_row; p.k_head = a.k_head; p.v_page = a.v_page; p.v_row = a.v_row; p.v_head = a.v_head;
+    p.sequences = a.sequences; p.chunk = a.chunk; p.rows = a.rows; p.k_ld = a.k_ld; p.v_ld = a.v_ld; p.kv_heads = a.kv_heads; p.dim = a.dim;
+    p.vdim = a.vdim; p.table_ld = a.table_ld; p.page_rows = a.page_rows; p.pool_pages = a.pool_pages;
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_paged_append(p, a.dtype, as_stream(stream));
+}
+
+uint64_t tnsr_b200_paged_attention_workspace(uint32_t dim, uint32_t vdim, int dtype) { return paged_attention_workspace_bytes(dim, vdim, dtype); }
+
+int tnsr_b200_paged_attention(const tnsr_b200_paged_attention_args* args, void* stream) {
+    tnsr_b200_paged_attention_args a;
+    if (const char* problem = paged_problem(args, a)) return bad_pages("paged_attention", problem);
+    if (!a.q || !a.out) return bad("paged_attention: null pointer");
+    if (a.heads == 0 || a.heads % a.kv_heads || a.q_ld < (uint64_t)a.heads * a.dim || a.out_ld < (uint64_t)a.heads * a.vdim)
+        return bad("paged_attention: kv_heads must divide heads, and rows must hold every head");
+    if (a.dim > 256 || a.vdim > 256) {
+        set_thread_error("paged_attention: widths are at most 256");
+        return TNSR_B200_ERR_UNSUPPORTED;
+    }
+    if (!std::isfinite(a.scale)) return bad("paged_attention: scale must be finite");
+    if (a.sinks && !a.window) return bad("paged_attention: sinks are the first keys beside a window");
+    if (a.workspace && (a.workspace_bytes < paged_attention_workspace_bytes(a.dim, a.vdim, a.dtype) || !aligned16(a.workspace)))
+        return bad("paged_attention: workspace smaller than tnsr_b200_paged_attention_workspace() asks for, or not 16-byte aligned");
+    PagedAttention p;
+    p.q = a.q; p.k_pool = a.k_pool; p.v_pool = a.v_pool; p.table = a.table; p.lengths = a.lengths; p.row_starts = a.row_starts; p.out = a.out;
+    p.workspace = a.workspace; p.d_status = a.d_status; p.workspace_bytes = a.workspace_bytes;
+    p.k_page = a.k_page; p.k_row = a.k_row; p.k_head = a.k_head; p.v_page = a.v_page; p.v_row = a.v_row; p.v_head = a.v_head;
+    p.sequences = a.sequences; p.chunk = a.chunk; p.rows = a.rows; p.q_ld = a.q_ld; p.out_ld = a.out_ld; p.heads = a.heads; p.kv_heads = a.kv_heads;
+    p.dim = a.dim; p.vdim = a.vdim; p.table_ld = a.table_ld; p.page_rows = a.page_rows; p.pool_pages = a.pool_pages; p.window = a.window;
+    p.sinks = a.sinks; p.scale = a.scale;
+    const OverlapLaunches overlap(as_stream(stream));
+    return launch_paged_attention(p, a.dtype, as_stream(stream));
 }
 
 }  // extern "C"

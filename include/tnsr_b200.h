@@ -905,7 +905,9 @@ TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args
  * bits for few rows, 8 bits for many.  Keys in a page outside the pool (status 4)
  * count as zeros.  Status 2: a bounded wait inside the kernel for many rows gave up.
  * workspace: tnsr_b200_paged_attention_workspace() bytes; NULL: the keys of a
- * sequence are not divided. */
+ * sequence are not divided.  The same call gives the same bits; where the keys of a
+ * sequence are divided, and with it the last bits of its sums, depends on the
+ * lengths of all of them. */
 typedef struct tnsr_b200_paged_attention_args {
     const void *q, *k_pool, *v_pool;
     const uint32_t *table, *lengths, *row_starts;

@@ -150,7 +150,9 @@ def test_bad_tables_and_lengths_are_reported_and_nothing_outside_is_read(dtype, 
     table = cache.host_table.copy()
     table[2] = 0
     got = cache.run(status=3, lengths=u32(lengths).data_ptr(), table=u32(table).data_ptr())
-    assert torch.equal(got[:int(cache.starts[2])], good[:int(cache.starts[2])])
+    # where keys are cut, and with it the last bits, follows all lengths: within the tolerance, not to the bit
+    want, tol = cache.expected()
+    assert bool(((got.double() - want).abs() <= tol)[:int(cache.starts[2])].all())
 
 
 def test_row_starts_that_lie_are_cut_to_the_rows_there_are():

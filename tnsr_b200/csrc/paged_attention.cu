@@ -80,7 +80,747 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(PagedParams p) {
     paged_row<T>(p, s, seq, row, h, threadIdx.x & 31);
 }
 
-uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype) { return 256; }
+// ---- few rows: keys divided over blocks -------------------------------------------------------------------------------------------
+// A unit is 16 rows (tokens x query heads) of one sequence and key/value head; its tiles are the TK keys each that some of the rows see: those of
+// the first keys, then those from the first row's window on.  All tiles of all units, one unit behind the other, are divided into equal runs,
+// a run per block, so that no block waits for a long sequence: a unit whose tiles lie in several runs leaves a partial result (numerators,
+// maximum, sum) per block, and the block that arrives last joins them in the order of the runs.  A block finds its run by itself from the
+// lengths (a prefix sum over the sequences), so nothing is planned on the host and a captured call follows its lengths.
+struct FewUnit {
+    PagedSequence seq;
+    uint32_t s, kvh, rt, row_tiles;
+    uint32_t row0, rows;         // first row and how many
+    int32_t first, last;         // positions of the first and the last row's token
+    uint32_t tiles, head_tiles, gap;    // tiles; those of the first keys; tile of the window's first key
+};
+
+template <uint32_t TK>
+__device__ __forceinline__ void unit_tiles(const PagedParams& p, FewUnit& u) {
+    u.row0 = u.rt * 16;
+    u.rows = min(16u, u.seq.count * p.per.d - u.row0);
+    const int32_t base = (int32_t)u.seq.length - (int32_t)u.seq.count;
+    u.first = base + (int32_t)p.per.div(u.row0);
+    u.last = base + (int32_t)p.per.div(u.row0 + u.rows - 1);
+    u.head_tiles = u.gap = 0;
+    if (u.last < 0) {            // nothing to see: one tile, all hidden, so that somebody writes the zeros
+        u.tiles = 1;
+        return;
+    }
+    if (p.a.window && u.first >= (int32_t)p.a.window) {
+        u.gap = (uint32_t)(u.first + 1 - (int32_t)p.a.window) / TK;
+        u.head_tiles = min((min(p.a.sinks, (uint32_t)u.last + 1) + TK - 1) / TK, u.gap);
+    }
+    u.tiles = u.head_tiles + (uint32_t)u.last / TK - u.gap + 1;
+}
+template <uint32_t TK>
+__device__ __forceinline__ void load_sequence(const PagedParams& p, FewUnit& u) {
+    u.seq = paged_sequence(p, u.s);
+    u.row_tiles = (u.seq.count * p.per.d + 15) / 16;
+}
+// Tiles of all units of one key/value head of the sequence.
+template <uint32_t TK>
+__device__ __forceinline__ uint32_t head_tiles(const PagedParams& p, FewUnit u) {
+    uint32_t n = 0;
+    for (u.rt = 0; u.rt < u.row_tiles; ++u.rt) {
+        unit_tiles<TK>(p, u);
+        n += u.tiles;
+    }
+    return n;
+}
+
+// Where a block stands: a unit and a tile of it.
+template <uint32_t TK>
+struct FewCursor {
+    FewUnit u;
+    uint32_t tile;
+    uint64_t at;                 // tiles before this one, of all units
+    __device__ __forceinline__ void next_unit(const PagedParams& p) {
+        tile = 0;
+        if (++u.rt == u.row_tiles) {
+            u.rt = 0;
+            if (++u.kvh == p.a.kv_heads) {
+                u.kvh = 0;
+                do {
+                    if (++u.s >= p.a.sequences) return;
+                    load_sequence<TK>(p, u);
+                } while (u.row_tiles == 0);
+            }
+        }
+        unit_tiles<TK>(p, u);
+    }
+    __device__ __forceinline__ void next(const PagedParams& p) {
+        ++at;
+        if (++tile == u.tiles) next_unit(p);
+    }
+    __device__ __forceinline__ uint32_t key0() const { return (tile < u.head_tiles ? tile : u.gap + tile - u.head_tiles) * TK; }
+};
+
+struct FewRun {
+    uint64_t begin, end, length;         // of this block; tiles of a run
+};
+
+// Prefix sums over 128 threads.
+__device__ __forceinline__ uint64_t scan128(uint64_t v, uint64_t* warps, uint64_t& total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) warps[warp] = x;
+    __syncthreads();
+    uint64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+        if (w < warp) before += warps[w];
+        total += warps[w];
+    }
+    return before + x - v;
+}
+
+// This block's run and its first tile; false: there is none.  `whole`: runs end where units do.
+template <uint32_t TK>
+__device__ __forceinline__ bool few_plan(const PagedParams& p, bool whole, FewRun& run, FewCursor<TK>& c) {
+    __shared__ uint64_t warps[4], s_at;
+    __shared__ uint32_t s_sequence;
+    const uint32_t share = (p.a.sequences + 127) / 128, s0 = min(p.a.sequences, threadIdx.x * share), s1 = min(p.a.sequences, s0 + share);
+    uint64_t mine = 0;
+    for (c.u.s = s0; c.u.s < s1; ++c.u.s) {
+        load_sequence<TK>(p, c.u);
+        mine += (uint64_t)head_tiles<TK>(p, c.u) * p.a.kv_heads;
+    }
+    uint64_t total;
+    uint64_t before = scan128(mine, warps, total);
+    run.length = max((uint64_t)1, (total + gridDim.x - 1) / gridDim.x);
+    run.begin = blockIdx.x * run.length;
+    run.end = min(total, run.begin + run.length);
+    if (run.begin >= total) return false;
+    if (run.begin >= before && run.begin < before + mine) {
+        for (c.u.s = s0; c.u.s < s1; ++c.u.s) {
+            load_sequence<TK>(p, c.u);
+            const uint64_t n = (uint64_t)head_tiles<TK>(p, c.u) * p.a.kv_heads;
+            if (run.begin < before + n) break;
+            before += n;
+        }
+        s_sequence = c.u.s;
+        s_at = before;
+    }
+    __syncthreads();
+    c.u.s = s_sequence;
+    load_sequence<TK>(p, c.u);
+    uint64_t rest = run.begin - s_at;
+    const uint32_t per_head = head_tiles<TK>(p, c.u);
+    c.u.kvh = (uint32_t)(rest / per_head);
+    uint32_t r = (uint32_t)(rest % per_head);
+    for (c.u.rt = 0;; ++c.u.rt) {
+        unit_tiles<TK>(p, c.u);
+        if (r < c.u.tiles) break;
+        r -= c.u.tiles;
+    }
+    c.tile = r;
+    c.at = run.begin;
+    if (whole && c.tile) {                       // the block before has this unit
+        c.at += c.u.tiles - c.tile;
+        c.next_unit(p);
+        if (c.at >= run.end) return false;
+    }
+    return true;
+}
+__device__ __forceinline__ bool row_sees(const PagedParams& p, int32_t at, uint32_t key) {
+    return (int32_t)key <= at && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > at);
+}
+// Whether any row of the unit sees the key: what nobody sees is not looked up.
+__device__ __forceinline__ bool unit_sees(const PagedParams& p, const FewUnit& u, uint32_t key) {
+    return (int32_t)key <= u.last && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > u.first);
+}
+
+constexpr uint32_t FEW_BLOCKS = 592;             // at the most
+constexpr uint32_t FEW_COUNTERS = 4096;          // bytes before the partial results
+static_assert(FEW_COUNTERS >= FEW_BLOCKS * 4, "a counter per block");
+
+// Partial results of a unit joined by the block that comes last, in the order of the runs.  Layout [block][whether the unit begins in its run][16][W + 2].
+// A warp per row; lanes hold the factors of 32 parts at a time.
+template <int W, typename T>
+__device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
+    __shared__ uint32_t s_last;
+    const uint32_t c0 = (uint32_t)(unit_at / run.length), c1 = (uint32_t)((unit_at + u.tiles - 1) / run.length), parts = c1 - c0 + 1;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(done + c0, 1u) + 1 == parts;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t r = threadIdx.x >> 5; r < u.rows; r += 4) {
+        auto part = [&](uint32_t i) { return partial + (((uint64_t)(c0 + i) * 2 + (i == 0)) * 16 + r) * (W + 2); };
+        float top = -INFINITY;
+        for (uint32_t i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(part(i) + W));
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float ms = top == -INFINITY ? 0.0f : top;
+        const uint32_t R = u.row0 + r, token = p.per.div(R), h = u.kvh * p.per.d + R - token * p.per.d;
+        T* out = reinterpret_cast<T*>(p.a.out) + (uint64_t)(u.seq.start + token) * p.a.out_ld + (uint64_t)h * p.a.vdim;
+        float2 v[W / 64];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W / 64; ++j) v[j] = make_float2(0.0f, 0.0f);
+        for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
+            const uint32_t n = min(32u, parts - i0);
+            const float factor = lane < n ? mx_ex2(__ldcg(part(i0 + lane) + W) - ms) : 0.0f;
+            if (lane < n) sum = fmaf(factor, __ldcg(part(i0 + lane) + W + 1), sum);
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; ++i) {
+                const float f = __shfl_sync(0xffffffffu, factor, i);
+                const float2* src = reinterpret_cast<const float2*>(part(i0 + i));
+#pragma unroll
+                for (int j = 0; j < W / 64; ++j) {
+                    const float2 x = __ldcg(src + j * 32 + lane);
+                    v[j].x = fmaf(f, x.x, v[j].x);
+                    v[j].y = fmaf(f, x.y, v[j].y);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int j = 0; j < W / 64; ++j) {
+            const uint32_t c = j * 64 + lane * 2;
+            if (c < p.a.vdim) out[c] = from_f32<T>(v[j].x * inv);
+            if (c + 1 < p.a.vdim) out[c + 1] = from_f32<T>(v[j].y * inv);
+        }
+    }
+    if (threadIdx.x == 0) done[c0] = 0;
+}
+
+// bf16 on mma.sync: a tile is 64 keys.  Scores: a warp has 16 keys and all 16 rows; the value product: a warp has a quarter of the columns and all
+// 64 keys, so that nothing is left to be added up between the warps but the sums of the weights.  Tiles arrive by 16-byte asynchronous
+// copies, STAGES - 1 of them ahead; lane l < 16 of a warp looks up the place of one of its 16 rows a tile before that is asked for.
+// Weights enter the value product as two bf16 pieces (16 bits): the kernel waits for memory, not for the tensor cores.
+// A tile that some rows see only in part may hold infinities or NaN in values that are hidden from others, which a weight of 0 does not
+// keep out: its values are looked through, and if there are any its product is made key by key for each row.
+// STAGES: three of 64 keys keep 64 KB per SM on their way with widths of 128 (two blocks per SM) and 64 (three).
+template <int W, int STAGES>
+struct FewShape {
+    static constexpr uint32_t PITCH = W * 2 + 16, TILE = 64 * PITCH, STAGE = 2 * TILE;
+    static constexpr uint32_t P_PITCH = 64 * 2 + 16, P_BYTES = 2 * 16 * P_PITCH;
+    static constexpr uint32_t BYTES = STAGES * STAGE + P_BYTES + 2 * 4 * 16 * 4;
+};
+
+template <int W, int STAGES, bool UPPER>
+__global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* partial, uint32_t* done) {
+    using S = FewShape<W, STAGES>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint8_t* weights = smem + STAGES * S::STAGE;
+    float* tops = reinterpret_cast<float*>(weights + S::P_BYTES);        // [4][16]
+    float* sums = tops + 64;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    pdl_trigger();
+    FewRun run;
+    FewCursor<64> ahead;
+    if (!few_plan<64>(p, partial == nullptr, run, ahead)) return;
+    FewCursor<64> c = ahead;
+    const PagedAttention& a = p.a;
+    // one unit at the end of the run, where runs end with units
+    auto over = [&](const FewCursor<64>& x) { return partial ? x.at >= run.end : x.at >= run.end && x.tile == 0; };
+
+    // row (lane / 2) * 8 + warp * 2 + lane % 2 of the tile ahead, lanes 0 .. 15: its page (or a mark that it is not wanted) and its row there
+    uint32_t page = PA_NONE, row = 0, kvh_ahead = 0;
+    bool wanted = false, more = true;
+    auto look_up = [&]() {
+        wanted = false;
+        more = !over(ahead);
+        if (!more) return;
+        const uint32_t key = ahead.key0() + (lane >> 1) * 8 + warp * 2 + (lane & 1);
+        kvh_ahead = ahead.u.kvh;
+        if (lane < 16 && unit_sees(p, ahead.u, key)) {
+            const uint32_t i = p.page.div(key);
+            row = key - i * p.page.d;
+            page = a.table[(uint64_t)ahead.u.s * a.table_ld + i];
+            wanted = true;
+        }
+        ahead.next(p);
+    };
+    constexpr uint32_t CH = W / 8;               // 16-byte pieces of a row
+    auto load = [&](uint32_t stage) {
+        if (more) {
+            uint64_t k_at = 0, v_at = 0;
+            bool real = wanted && page < a.pool_pages;
+            if (wanted && !real) report(a.d_status, DEV_BAD_PAGE);
+            if (real) {
+                k_at = a.k_page * page + a.k_row * row + a.k_head * kvh_ahead;
+                v_at = a.v_page * page + a.v_row * row + a.v_head * kvh_ahead;
+            }
+            uint8_t* dst = smem + stage * S::STAGE;
+            // the warp copies its own 16 rows, 32 / CH of them at a time
+#pragma unroll
+            for (uint32_t i = 0; i < 16 * CH / 32; ++i) {
+                const uint32_t piece = i * 32 + lane, owner = piece / CH, ch = piece % CH;
+                const uint64_t k_row = __shfl_sync(0xffffffffu, k_at, owner), v_row = __shfl_sync(0xffffffffu, v_at, owner);
+                const bool there = __shfl_sync(0xffffffffu, (int)real, owner);
+                const uint32_t r = (owner >> 1) * 8 + warp * 2 + (owner & 1);
+                mx_cp16(dst + r * S::PITCH + ch * 16, reinterpret_cast<const bf16*>(a.k_pool) + k_row + (there && ch * 8 < a.dim ? ch * 8 : 0),
+                        there && ch * 8 < a.dim);
+                mx_cp16(dst + S::TILE + r * S::PITCH + ch * 16, reinterpret_cast<const bf16*>(a.v_pool) + v_row + (there && ch * 8 < a.vdim ? ch * 8 : 0),
+                        there && ch * 8 < a.vdim);
+            }
+        }
+        mx_commit();
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        load(i);
+        look_up();
+    }
+
+    uint32_t qa[W / 16][4];
+    float o[W / 32][4], m0, m1, l0, l1;
+    int32_t at0, at1;                    // positions of rows g8 and g8 + 8
+    uint64_t unit_at = c.at - c.tile;
+    auto begin_unit = [&]() {
+        unit_at = c.at - c.tile;
+        const int32_t base = (int32_t)c.u.seq.length - (int32_t)c.u.seq.count;
+        auto place = [&](uint32_t r, uint32_t& token) {
+            const uint32_t R = c.u.row0 + min(r, c.u.rows - 1);
+            token = p.per.div(R);
+            return c.u.kvh * p.per.d + R - token * p.per.d;
+        };
+        uint32_t token0, token1;
+        const uint32_t h0 = place(g8, token0), h1 = place(g8 + 8, token1);
+        at0 = base + (int32_t)token0;
+        at1 = base + (int32_t)token1;
+        const bf16* q0 = reinterpret_cast<const bf16*>(a.q) + (uint64_t)(c.u.seq.start + token0) * a.q_ld + (uint64_t)h0 * a.dim;
+        const bf16* q1 = reinterpret_cast<const bf16*>(a.q) + (uint64_t)(c.u.seq.start + token1) * a.q_ld + (uint64_t)h1 * a.dim;
+        auto pair = [&](const bf16* q, uint32_t col) { return col < a.dim ? *reinterpret_cast<const uint32_t*>(q + col) : 0u; };
+#pragma unroll
+        for (int k = 0; k < W / 16; ++k) {
+            qa[k][0] = pair(q0, k * 16 + t4 * 2);
+            qa[k][1] = UPPER ? pair(q1, k * 16 + t4 * 2) : 0u;
+            qa[k][2] = pair(q0, k * 16 + 8 + t4 * 2);
+            qa[k][3] = UPPER ? pair(q1, k * 16 + 8 + t4 * 2) : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < W / 32; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.0f;
+    };
+    auto end_unit = [&]() {
+        // sums of the weights over a row's four lanes and the four warps
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        if (UPPER) {
+            l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        }
+        if (t4 == 0) {
+            sums[warp * 16 + g8] = l0;
+            if (UPPER) sums[warp * 16 + g8 + 8] = l1;
+        }
+        __syncthreads();
+        const bool all = unit_at >= run.begin && c.tile + 1 == c.u.tiles;      // c stands at the unit's last tile in this run
+#pragma unroll
+        for (int half = 0; half < (UPPER ? 2 : 1); ++half) {
+            const uint32_t r = g8 + half * 8;
+            if (r >= c.u.rows) continue;
+            const float l = sums[r] + sums[16 + r] + sums[32 + r] + sums[48 + r];
+            if (all) {
+                const uint32_t R = c.u.row0 + r, token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                bf16* out = reinterpret_cast<bf16*>(a.out) + (uint64_t)(c.u.seq.start + token) * a.out_ld + (uint64_t)h * a.vdim;
+#pragma unroll
+                for (int n = 0; n < W / 32; ++n) {
+                    const uint32_t col = warp * (W / 4) + n * 8 + t4 * 2;
+                    if (col < a.vdim) *reinterpret_cast<uint32_t*>(out + col) = pack_bf16x2(o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
+                }
+            } else {
+                float* dst = partial + (((uint64_t)blockIdx.x * 2 + (unit_at >= run.begin)) * 16 + r) * (W + 2);
+#pragma unroll
+                for (int n = 0; n < W / 32; ++n)
+                    *reinterpret_cast<float2*>(dst + warp * (W / 4) + n * 8 + t4 * 2) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+                if (warp == 0 && t4 == 0) {
+                    dst[W] = half ? m1 : m0;
+                    dst[W + 1] = l;
+                }
+            }
+        }
+        return all;
+    };
+    begin_unit();
+    uint32_t stage = 0;
+    while (true) {
+        mx_wait<STAGES - 2>();
+        __syncthreads();
+        load((stage + STAGES - 1) % STAGES);         // where the tile before this one was
+        look_up();
+        const uint8_t* tile = smem + stage * S::STAGE;
+        const uint32_t sk = mx_smem(tile), sv = sk + S::TILE, key0 = c.key0();
+        float sc[2][4] = {}, odd[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < W / 16; k += 2) {
+            uint32_t b[4], d[4];
+            const uint32_t at = sk + (warp * 16 + (lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16 + k * 32;
+            mx_ldsm(at, b);
+            mx_ldsm(at + 32, d);
+            mx_mma(sc[0], qa[k], b[0], b[1]);
+            mx_mma(sc[1], qa[k], b[2], b[3]);
+            mx_mma(odd[0], qa[k + 1], d[0], d[1]);
+            mx_mma(odd[1], qa[k + 1], d[2], d[3]);
+        }
+        const bool partly = (int64_t)key0 + 63 > c.u.first || (a.window && (int64_t)key0 + a.window <= c.u.last);
+        float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < (UPPER ? 4 : 2); ++e) {
+                float v = (sc[n][e] + odd[n][e]) * p.scale_log2;
+                if (partly && !row_sees(p, e < 2 ? at0 : at1, key0 + warp * 16 + n * 8 + t4 * 2 + (e & 1))) v = -INFINITY;
+                sc[n][e] = v;
+                if (e < 2) top0 = fmaxf(top0, v); else top1 = fmaxf(top1, v);
+            }
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
+        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
+        if (UPPER) {
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+        }
+        if (t4 == 0) {
+            tops[warp * 16 + g8] = top0;
+            if (UPPER) tops[warp * 16 + g8 + 8] = top1;
+        }
+        __syncthreads();
+        auto weigh = [&](int half, float& m, float& l) {
+            const float* t = tops + half * 8 + g8;
+            const float top = fmaxf(fmaxf(m, fmaxf(t[0], t[16])), fmaxf(t[32], t[48])), ms = top == -INFINITY ? 0.0f : top, f = mx_ex2(m - ms);
+            m = top;
+            float sum = 0.0f;
+            uint8_t* dst = weights + (half * 8 + g8) * S::P_PITCH + (warp * 16 + t4 * 2) * 2;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float x = mx_ex2(sc[n][2 * half] - ms), y = mx_ex2(sc[n][2 * half + 1] - ms);
+                sum += x + y;
+                uint32_t hi, lo;
+                split_bf16x2(x, y, hi, lo);
+                *reinterpret_cast<uint32_t*>(dst + n * 16) = hi;
+                *reinterpret_cast<uint32_t*>(dst + 16 * S::P_PITCH + n * 16) = lo;
+            }
+            l = l * f + sum;
+#pragma unroll
+            for (int n = 0; n < W / 32; ++n) {
+                o[n][2 * half] *= f;
+                o[n][2 * half + 1] *= f;
+            }
+        };
+        weigh(0, m0, l0);
+        if (UPPER) weigh(1, m1, l1);
+        // values that some rows see and others do not
+        bool odd_values = false;
+        if (partly && c.u.first != c.u.last) {
+            for (uint32_t i = threadIdx.x; i < 64 * CH; i += 128) {
+                const uint4 v = *reinterpret_cast<const uint4*>(tile + S::TILE + (i / CH) * S::PITCH + (i % CH) * 16);
+                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd_values |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
+            }
+        }
+        if (__syncthreads_or(odd_values)) {
+            for (uint32_t j = 0; j < 64; ++j) {
+#pragma unroll
+                for (int half = 0; half < (UPPER ? 2 : 1); ++half) {
+                    if (!row_sees(p, half ? at1 : at0, key0 + j)) continue;
+                    const uint8_t* w = weights + (half * 8 + g8) * S::P_PITCH + j * 2;
+                    const float x = __bfloat162float(*reinterpret_cast<const bf16*>(w)) + __bfloat162float(*reinterpret_cast<const bf16*>(w + 16 * S::P_PITCH));
+#pragma unroll
+                    for (int n = 0; n < W / 32; ++n) {
+                        const float2 v = bf16x2_to_f32(*reinterpret_cast<const uint32_t*>(tile + S::TILE + j * S::PITCH + (warp * (W / 4) + n * 8 + t4 * 2) * 2));
+                        o[n][2 * half] = fmaf(x, v.x, o[n][2 * half]);
+                        o[n][2 * half + 1] = fmaf(x, v.y, o[n][2 * half + 1]);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t hi[4], lo[4];
+                const uint32_t wa = mx_smem(weights) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::P_PITCH + k * 32 + (lane >> 4) * 16;
+                mx_ldsm(wa, hi);
+                mx_ldsm(wa + 16 * S::P_PITCH, lo);
+                if (!UPPER) hi[1] = hi[3] = lo[1] = lo[3] = 0;
+#pragma unroll
+                for (int n = 0; n < W / 64; ++n) {
+                    uint32_t b[4];
+                    mx_ldsm_t(sv + (k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (warp * (W / 4) + n * 16 + (lane >> 4) * 8) * 2, b);
+                    mx_mma(o[2 * n], hi, b[0], b[1]);
+                    mx_mma(o[2 * n + 1], hi, b[2], b[3]);
+                    mx_mma(o[2 * n], lo, b[0], b[1]);
+                    mx_mma(o[2 * n + 1], lo, b[2], b[3]);
+                }
+            }
+        }
+        stage = (stage + 1) % STAGES;
+        const bool unit_over = c.tile + 1 == c.u.tiles, run_over = partial ? c.at + 1 >= run.end : unit_over && c.at + 1 >= run.end;
+        if (unit_over || run_over) {
+            if (!end_unit()) few_join<W, bf16>(p, c.u, unit_at, run, partial, done);
+            if (run_over) break;
+        }
+        c.next(p);
+        if (unit_over) begin_unit();
+    }
+    mx_wait<0>();
+}
+
+// f32 on CUDA cores: a tile is 32 keys.  Scores: a thread has a key and the rows warp, warp + 4, ...; the value product: a thread has a column (two
+// at widths of 256; half the keys at 64) and all rows.  RQ: rows of a warp.
+template <int W, int STAGES>
+struct FewShape32 {
+    static constexpr uint32_t PITCH = W * 4 + 16, TILE = 32 * PITCH, STAGE = 2 * TILE;
+    static constexpr uint32_t Q = STAGES * STAGE, P = Q + 16 * W * 4, BYTES = P + 32 * 16 * 4 + (W == 64 ? 64 * 16 * 4 : 0) + 4 * 64;
+};
+
+template <int W, int STAGES, int RQ>
+__global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float* partial, uint32_t* done) {
+    using S = FewShape32<W, STAGES>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* sq = reinterpret_cast<float*>(smem + S::Q);
+    float* weights = reinterpret_cast<float*>(smem + S::P);              // [32 keys][16 rows]
+    float* half_sums = weights + 32 * 16;                                // W == 64: [16][64]
+    float* factors = half_sums + (W == 64 ? 64 * 16 : 0);                // [16] each: factors, sums, maxima, positions
+    float *sums = factors + 16, *tops = sums + 16;
+    int32_t* places = reinterpret_cast<int32_t*>(tops + 16);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_trigger();
+    FewRun run;
+    FewCursor<32> ahead;
+    if (!few_plan<32>(p, partial == nullptr, run, ahead)) return;
+    FewCursor<32> c = ahead;
+    const PagedAttention& a = p.a;
+    auto over = [&](const FewCursor<32>& x) { return partial ? x.at >= run.end : x.at >= run.end && x.tile == 0; };
+
+    // row warp * 8 + lane of the tile ahead, lanes 0 .. 7
+    uint32_t page = PA_NONE, row = 0, kvh_ahead = 0;
+    bool wanted = false, more = true;
+    auto look_up = [&]() {
+        wanted = false;
+        more = !over(ahead);
+        if (!more) return;
+        const uint32_t key = ahead.key0() + warp * 8 + lane;
+        kvh_ahead = ahead.u.kvh;
+        if (lane < 8 && unit_sees(p, ahead.u, key)) {
+            const uint32_t i = p.page.div(key);
+            row = key - i * p.page.d;
+            page = a.table[(uint64_t)ahead.u.s * a.table_ld + i];
+            wanted = true;
+        }
+        ahead.next(p);
+    };
+    constexpr uint32_t CH = W / 4;
+    auto load = [&](uint32_t stage) {
+        if (more) {
+            uint64_t k_at = 0, v_at = 0;
+            const bool real = wanted && page < a.pool_pages;
+            if (wanted && !real) report(a.d_status, DEV_BAD_PAGE);
+            if (real) {
+                k_at = a.k_page * page + a.k_row * row + a.k_head * kvh_ahead;
+                v_at = a.v_page * page + a.v_row * row + a.v_head * kvh_ahead;
+            }
+            uint8_t* dst = smem + stage * S::STAGE + warp * 8 * S::PITCH;
+#pragma unroll
+            for (uint32_t i = 0; i < 8 * CH / 32; ++i) {
+                const uint32_t piece = i * 32 + lane, owner = piece / CH, ch = piece % CH;
+                const uint64_t k_row = __shfl_sync(0xffffffffu, k_at, owner), v_row = __shfl_sync(0xffffffffu, v_at, owner);
+                const bool there = __shfl_sync(0xffffffffu, (int)real, owner);
+                mx_cp16(dst + owner * S::PITCH + ch * 16, reinterpret_cast<const float*>(a.k_pool) + k_row + (there && ch * 4 < a.dim ? ch * 4 : 0),
+                        there && ch * 4 < a.dim);
+                mx_cp16(dst + S::TILE + owner * S::PITCH + ch * 16, reinterpret_cast<const float*>(a.v_pool) + v_row + (there && ch * 4 < a.vdim ? ch * 4 : 0),
+                        there && ch * 4 < a.vdim);
+            }
+        }
+        mx_commit();
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        load(i);
+        look_up();
+    }
+
+    constexpr int COLUMNS = W == 256 ? 2 : 1, KEYS = W == 64 ? 16 : 32;   // of a thread in the value product
+    const uint32_t col = tid % W, key_first = W == 64 ? (tid / 64) * 16 : 0;
+    float o[COLUMNS][RQ * 4], m[RQ], l[RQ];
+    uint64_t unit_at = c.at - c.tile;
+    auto begin_unit = [&]() {
+        unit_at = c.at - c.tile;
+        __syncthreads();                     // the last unit's rows are done with
+        const int32_t base = (int32_t)c.u.seq.length - (int32_t)c.u.seq.count;
+        for (uint32_t i = tid; i < RQ * 4 * W; i += 128) {
+            const uint32_t r = i / W, x = i % W, R = c.u.row0 + min(r, c.u.rows - 1), token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
+            sq[i] = r < c.u.rows && x < a.dim
+                        ? reinterpret_cast<const float*>(a.q)[(uint64_t)(c.u.seq.start + token) * a.q_ld + (uint64_t)h * a.dim + x] * p.scale_log2 : 0.0f;
+            if (x == 0) places[r] = base + (int32_t)token;
+        }
+#pragma unroll
+        for (int i = 0; i < RQ * 4; ++i)
+#pragma unroll
+            for (int n = 0; n < COLUMNS; ++n) o[n][i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+        }
+    };
+    auto end_unit = [&]() {
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            float sum = l[i];
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane == 0) {
+                sums[warp + 4 * i] = sum;
+                tops[warp + 4 * i] = m[i];
+            }
+        }
+        if (W == 64 && tid >= 64)
+#pragma unroll
+            for (int r = 0; r < RQ * 4; ++r) half_sums[r * 64 + col] = o[0][r];
+        __syncthreads();
+        const bool all = unit_at >= run.begin && c.tile + 1 == c.u.tiles;
+        if (W != 64 || tid < 64) {
+#pragma unroll
+            for (int r = 0; r < RQ * 4; ++r) {
+                if (r >= c.u.rows) continue;
+                const uint32_t R = c.u.row0 + r, token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
+                const float inv = sums[r] == 0.0f ? 0.0f : 1.0f / sums[r];
+                float* out = reinterpret_cast<float*>(a.out) + (uint64_t)(c.u.seq.start + token) * a.out_ld + (uint64_t)h * a.vdim;
+                float* dst = partial + (((uint64_t)blockIdx.x * 2 + (unit_at >= run.begin)) * 16 + r) * (W + 2);
+#pragma unroll
+                for (int n = 0; n < COLUMNS; ++n) {
+                    const uint32_t x = col + n * 128;
+                    const float v = W == 64 ? o[n][r] + half_sums[r * 64 + col] : o[n][r];
+                    if (!all) dst[x] = v;
+                    else if (x < a.vdim) out[x] = v * inv;
+                }
+                if (!all && tid == 0) {
+                    dst[W] = tops[r];
+                    dst[W + 1] = sums[r];
+                }
+            }
+        }
+        return all;
+    };
+    begin_unit();
+    uint32_t stage = 0;
+    while (true) {
+        mx_wait<STAGES - 2>();
+        __syncthreads();
+        load((stage + STAGES - 1) % STAGES);
+        look_up();
+        const uint8_t* tile = smem + stage * S::STAGE;
+        const uint32_t key0 = c.key0();
+        float dot[RQ] = {};
+        const float4* k = reinterpret_cast<const float4*>(tile + lane * S::PITCH);
+#pragma unroll 8
+        for (int x = 0; x < W / 4; ++x) {
+            const float4 kv = k[x];
+#pragma unroll
+            for (int i = 0; i < RQ; ++i) {
+                const float4 q = reinterpret_cast<const float4*>(sq + (warp + 4 * i) * W)[x];
+                dot[i] = fmaf(q.x, kv.x, fmaf(q.y, kv.y, fmaf(q.z, kv.z, fmaf(q.w, kv.w, dot[i]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RQ; ++i) {
+            const float x = row_sees(p, places[warp + 4 * i], key0 + lane) ? dot[i] : -INFINITY;
+            float top = fmaxf(m[i], x);
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float ms = top == -INFINITY ? 0.0f : top, f = exp2f(m[i] - ms), w = exp2f(x - ms);
+            m[i] = top;
+            l[i] = l[i] * f + w;
+            weights[lane * 16 + warp + 4 * i] = w;
+            if (lane == 0) factors[warp + 4 * i] = f;
+        }
+        bool odd_values = false;
+        if (c.u.first != c.u.last && ((int64_t)key0 + 31 > c.u.first || (a.window && (int64_t)key0 + a.window <= c.u.last)))
+            for (uint32_t i = tid; i < 32 * W; i += 128) odd_values |= !isfinite(reinterpret_cast<const float*>(tile + S::TILE + (i / W) * S::PITCH)[i % W]);
+        const bool careful = __syncthreads_or(odd_values);
+#pragma unroll
+        for (int r = 0; r < RQ * 4; ++r)
+#pragma unroll
+            for (int n = 0; n < COLUMNS; ++n) o[n][r] *= factors[r];
+#pragma unroll 4
+        for (int j = 0; j < KEYS; ++j) {
+            float v[COLUMNS];
+#pragma unroll
+            for (int n = 0; n < COLUMNS; ++n) v[n] = reinterpret_cast<const float*>(tile + S::TILE + (key_first + j) * S::PITCH)[col + n * 128];
+            const float4* w = reinterpret_cast<const float4*>(weights + (key_first + j) * 16);
+#pragma unroll
+            for (int q = 0; q < RQ; ++q) {
+                const float4 x = w[q];
+                const float f[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!careful || row_sees(p, places[4 * q + e], key0 + key_first + j))
+#pragma unroll
+                        for (int n = 0; n < COLUMNS; ++n) o[n][4 * q + e] = fmaf(f[e], v[n], o[n][4 * q + e]);
+            }
+        }
+        stage = (stage + 1) % STAGES;
+        const bool unit_over = c.tile + 1 == c.u.tiles, run_over = partial ? c.at + 1 >= run.end : unit_over && c.at + 1 >= run.end;
+        if (unit_over || run_over) {
+            if (!end_unit()) few_join<W, float>(p, c.u, unit_at, run, partial, done);
+            if (run_over) break;
+        }
+        c.next(p);
+        if (unit_over) begin_unit();
+    }
+    mx_wait<0>();
+}
+
+// ---- launch ------------------------------------------------------------------------------------------------------------------------
+namespace {
+constexpr int FEW_STAGES = 3;
+
+uint32_t few_width(uint32_t dim, uint32_t vdim) {
+    const uint32_t w = std::max(dim, vdim);
+    return w <= 64 ? 64 : w <= 128 ? 128 : 256;
+}
+// As many blocks as run at once: shared memory lets three (widths of 64), two or one of them on an SM.
+uint32_t few_blocks(uint32_t width) { return 148 * (width == 64 ? 3 : width == 128 ? 2 : 1); }
+
+template <auto KERNEL>
+int launch_few(const PagedParams& p, uint32_t bytes, uint32_t grid, cudaStream_t stream) {
+    if (const int rc = allow_shared<KERNEL>(bytes, "paged_attention attribute")) return rc;
+    float* partial = nullptr;
+    uint32_t* done = nullptr;
+    if (p.a.workspace) {
+        done = reinterpret_cast<uint32_t*>(p.a.workspace);
+        partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + FEW_COUNTERS);
+    }
+    launch_kernel(KERNEL, dim3(grid), dim3(128), bytes, stream, p, partial, done);
+    return TNSR_B200_OK;
+}
+template <int W>
+int launch_few_width(const PagedParams& p, int dtype, uint32_t rows, uint32_t grid, cudaStream_t stream) {
+    if (dtype == TNSR_B200_BF16) {
+        constexpr uint32_t bytes = FewShape<W, FEW_STAGES>::BYTES;
+        return rows > 8 ? launch_few<paged_few_kernel<W, FEW_STAGES, true>>(p, bytes, grid, stream)
+                        : launch_few<paged_few_kernel<W, FEW_STAGES, false>>(p, bytes, grid, stream);
+    }
+    constexpr uint32_t bytes = FewShape32<W, FEW_STAGES>::BYTES;
+    return rows > 8   ? launch_few<paged_few_f32_kernel<W, FEW_STAGES, 4>>(p, bytes, grid, stream)
+           : rows > 4 ? launch_few<paged_few_f32_kernel<W, FEW_STAGES, 2>>(p, bytes, grid, stream)
+                      : launch_few<paged_few_f32_kernel<W, FEW_STAGES, 1>>(p, bytes, grid, stream);
+}
+}  // namespace
+
+uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype) {
+    const uint32_t w = few_width(dim, vdim);
+    return FEW_COUNTERS + (uint64_t)few_blocks(w) * 2 * 16 * (w + 2) * 4;
+}
 
 int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stream) {
     if (a.rows == 0 || a.sequences == 0) return TNSR_B200_OK;
@@ -90,9 +830,27 @@ int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stre
     p.per = fast_div(a.heads / a.kv_heads);
     p.capacity = (uint32_t)std::min<uint64_t>((uint64_t)a.table_ld * a.page_rows, PAGED_MAX_KEYS);
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    const dim3 grid((unsigned)ceil_div64((uint64_t)a.rows * a.heads, 4));
-    if (dtype == TNSR_B200_F32) launch_kernel(paged_rows_kernel<float>, grid, dim3(128), 0, stream, p);
-    else launch_kernel(paged_rows_kernel<bf16>, grid, dim3(128), 0, stream, p);
+    // the other kernels copy 16 bytes at a time, and write pairs of columns
+    const uint32_t per = dtype == TNSR_B200_F32 ? 4 : 8;
+    const uint64_t strides = (uint64_t)a.dim | a.vdim | a.k_page | a.k_row | a.k_head | a.v_page | a.v_row | a.v_head;
+    const bool wide = strides % per == 0 && ((uintptr_t)a.k_pool | (uintptr_t)a.v_pool) % 16 == 0 &&
+                      (a.q_ld | a.out_ld) % 2 == 0 && ((uintptr_t)a.q | (uintptr_t)a.out) % 8 == 0;
+    const uint64_t rows = (uint64_t)a.chunk * p.per.d;
+    int rc = TNSR_B200_OK;
+    if (!wide || rows > 0x7fffffffu) {
+        const dim3 grid((unsigned)ceil_div64((uint64_t)a.rows * a.heads, 4));
+        if (dtype == TNSR_B200_F32) launch_kernel(paged_rows_kernel<float>, grid, dim3(128), 0, stream, p);
+        else launch_kernel(paged_rows_kernel<bf16>, grid, dim3(128), 0, stream, p);
+    } else {
+        const uint32_t w = few_width(a.dim, a.vdim), most = (uint32_t)std::min<uint64_t>(16, rows);
+        // no more blocks than there can be tiles
+        const uint64_t tiles = (uint64_t)a.sequences * a.kv_heads * ceil_div64(rows, 16) * (ceil_div(p.capacity, dtype == TNSR_B200_F32 ? 32u : 64u) + 1);
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, few_blocks(w));
+        rc = w == 64    ? launch_few_width<64>(p, dtype, most, grid, stream)
+             : w == 128 ? launch_few_width<128>(p, dtype, most, grid, stream)
+                        : launch_few_width<256>(p, dtype, most, grid, stream);
+    }
+    if (rc) return rc;
     count_launch();
     return check_launch("paged_attention");
 }

@@ -195,6 +195,24 @@ def test_same_bits_again_on_another_stream_in_a_graph_and_with_a_used_workspace(
     cache.check(cache.run(None))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_behind_one_another_whose_items_have_one_tile_or_two(dim):
+    """Calls on two caches in turn, without waiting: blocks of the grid go from items of one tile to items of two, on shared memory of all kinds of contents."""
+    caches = [Cache([1664, 512, 1280, 896, 2048], [259, 388, 648, 518, 777], 8, 2, dim, dim, 64, "bf16", seed=5, window=512, sinks=4),
+              Cache([100, 400, 90], [100, 70, 33], 4, 4, dim, dim, 16, "bf16", seed=6)]
+    want = [c.run().clone() for c in caches]
+    caches[1].check(want[1])
+    calls = [c.args() for c in caches]
+    for _ in range(30):
+        for c in caches:
+            c.out.fill_(-7.0)
+        for args in calls:
+            ok(lib().tnsr_b200_paged_attention(C.byref(args), stream()))
+        torch.cuda.synchronize()
+        for c, w in zip(caches, want):
+            assert torch.equal(c.out[:c.rows].float().cpu(), w)
+
+
 def test_many_sequences_and_one_long_one_beside_short_ones():
     rng = np.random.default_rng(0)
     lengths = list(rng.integers(0, 40, 700)) + [5000]

@@ -27,7 +27,7 @@ SOURCES = ["decoder.cu", "ops_api.cu", "elementwise.cu", "strict.cu", "strict_st
            "decode_attention_static.cu", "sampler.cu", "encoder.cu", "gemm_stream.cu",
            "layer_stack.cu", "mixer_attention.cu", "grouped_attention.cu", "mixer_mamba2.cu", "ssd_scan.cu", "mixer_hgrn2.cu", "hgrn2_scan.cu",
            "mixer_rglru.cu", "feed_forward.cu", "gemm_grouped.cu", "gemm_few.cu", "beam_select.cu", "pages.cu",
-           "paged_attention.cu"]
+           "paged_attention.cu", "paged_prompt.cu"]
 EXTRA = {name: ["--fmad=false"] for name in ("strict.cu", "strict_step.cu", "encoder.cu")}
 
 BASE_FLAGS = [

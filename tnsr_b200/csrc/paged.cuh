@@ -86,12 +86,57 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedParams& p, ui
     }
     return q;
 }
-// Place in the pool of key `key` (row of all pages in order), or ~0ull if its page lies outside.
+// Page of key `key` and its row there; false: no page of the pool.
 __device__ __forceinline__ bool paged_key(const PagedParams& p, const uint32_t* entries, uint32_t key, uint32_t& page, uint32_t& row) {
     const uint32_t i = p.page.div(key);
     row = key - i * p.page.d;
     page = entries[i];
     return page < p.a.pool_pages;
+}
+// One row and head by a warp, keys one by one: any widths, strides and alignment.
+template <typename T>
+__device__ __forceinline__ void paged_row(const PagedParams& p, uint32_t s, const PagedSequence& seq, uint32_t row, uint32_t h, uint32_t lane) {
+    const PagedAttention& a = p.a;
+    constexpr int N = 8;                         // 32 x 8 columns
+    const T* q = reinterpret_cast<const T*>(a.q) + (uint64_t)row * a.q_ld + (uint64_t)h * a.dim;
+    const uint32_t kvh = p.per.div(h), i = row - seq.start;
+    float qv[N], acc[N] = {};
+#pragma unroll
+    for (int n = 0; n < N; ++n) qv[n] = n * 32 + lane < a.dim ? to_f32(q[n * 32 + lane]) : 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int64_t at = (int64_t)seq.length - seq.count + i;
+    const uint32_t* entries = a.table + (uint64_t)s * a.table_ld;
+    const uint32_t keys = at < 0 ? 0u : (uint32_t)at + 1, first = a.window && keys > a.window ? keys - a.window : 0u;
+    for (uint32_t j = 0; j < keys; ++j) {
+        if (j < first && j >= a.sinks) {
+            j = first;                           // first <= at < keys
+        }
+        uint32_t page, r;
+        const bool real = paged_key(p, entries, j, page, r);
+        if (!real && lane == 0) report(a.d_status, DEV_BAD_PAGE);
+        const T* k = reinterpret_cast<const T*>(a.k_pool) + a.k_page * (real ? page : 0) + a.k_row * r + a.k_head * kvh;
+        const T* v = reinterpret_cast<const T*>(a.v_pool) + a.v_page * (real ? page : 0) + a.v_row * r + a.v_head * kvh;
+        float dot = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (real && n * 32 + lane < a.dim) dot = fmaf(qv[n], to_f32(k[n * 32 + lane]), dot);
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        const float x = dot * p.scale_log2, top = fmaxf(m, x), ms = top == -INFINITY ? 0.0f : top;
+        const float w = exp2f(x - ms), c = exp2f(m - ms);
+        m = top;
+        l = l * c + w;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const float y = real && n * 32 + lane < a.vdim ? to_f32(v[n * 32 + lane]) : 0.0f;
+            acc[n] = fmaf(w, y, acc[n] * c);
+        }
+    }
+    T* out = reinterpret_cast<T*>(a.out) + (uint64_t)row * a.out_ld + (uint64_t)h * a.vdim;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        if (n * 32 + lane < a.vdim) out[n * 32 + lane] = from_f32<T>(l == 0.0f ? 0.0f : acc[n] * inv);
 }
 #endif
 

@@ -1,0 +1,556 @@
+// Attention over pages for many rows per sequence, on tcgen05: bf16, widths up to 128 (multiples of 8).
+//
+// A tile is 128 rows (as many tokens as fit, times the query heads that share a key/value head), one TMEM lane each; an item is two tiles
+// of one sequence and key/value head that walk the same key blocks of 128 and take turns on the tensor cores: while one tile's
+// scores are turned into weights, the other's products run.  Blocks that no row of a tile sees are left out for it, those that no row of the
+// item sees are not read.
+//
+//   warp 0        TMA: per item the two query tiles, then blocks of keys and values into rings.  Pools are tensors {width, head, row, page}
+//                 of any strides; a box is the largest power of two of rows that divides a page, lane i of the warp looks box i's page up and asks for
+//                 it.  Boxes that are not wanted, or whose page lies outside the pool, get coordinates outside: zeros.
+//   warp 1        one thread issues S = Q K^T (128 x 128) and O += P V (128 x W), per tile: P V of block j, then S of block j + 1.
+//   warps 4-7, 8-11   softmax of tile 0 and 1, a thread per row: no exchange between threads.  The row's weights go back over its
+//                 scores as bf16 (the A operand in TMEM).  O stays in TMEM through an item and is rescaled only when a row's maximum has
+//                 grown by more than 2^8 since the last time (weights then are at most 2^8, sums f32); S of block j is complete only when
+//                 P V of block j - 1 is, so the rescaling needs no barrier of its own.
+//
+// Values that some rows of an item see and others do not may hold infinities or NaN, which a weight of 0 does not keep out, and so may the
+// rest of a last page: in blocks that are not seen by all, each row of values is looked through and such elements are zeroed before the
+// product; rows that see one of them are computed once more key by key.
+//
+// Every wait is bounded as elsewhere: one that gives up raises the abort flag, the roles fall through and the status word is set.
+#include <algorithm>
+
+#include "mixers.cuh"
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace tb {
+
+constexpr uint32_t PP_THREADS = 384;
+constexpr uint32_t PP_ODD = 16;                      // keys with values of no finite number that a tile remembers
+constexpr uint32_t PP_HALF = 128 * 128;              // 128 rows of 64 bf16
+
+template <int W>
+struct PromptShape {
+    static constexpr uint32_t TILE = PP_HALF * (W / 64);                // 128 rows of W
+    static constexpr uint32_t STAGES = W == 128 ? 2 : 4;
+    static constexpr uint32_t BYTES = 1024 + 2 * TILE + STAGES * 2 * TILE + 1024;
+};
+constexpr uint32_t PP_TMEM = 512;                    // scores 2 x 128, outputs 2 x W
+constexpr uint32_t PP_O = 256;
+
+constexpr uint32_t PP_IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+template <int W>
+constexpr uint32_t PP_IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)W >> 3) << 17) | ((128u >> 4) << 24);
+
+struct PromptParams {
+    PagedParams p;
+    uint32_t tokens;             // of a tile
+    uint32_t pairs;              // items of a sequence and key/value head at the most
+    uint32_t box;                // rows of a key box
+    uint64_t wait_limit_ns;
+};
+
+__device__ __forceinline__ void pp_mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void pp_st32(uint32_t taddr, const float* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    pp_st16(taddr, r);
+    pp_st16(taddr + 16, r + 16);
+}
+__device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pp_load_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void pp_load_4d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// Two tiles of a sequence and key/value head.
+struct PromptItem {
+    PagedSequence seq;
+    uint32_t s, kvh, token0;             // first token of the first tile
+    uint32_t tokens[2];                  // of each tile
+    int32_t first[2], last[2];           // positions of a tile's first and last token
+    int32_t low, high;                   // of the item's
+    uint32_t blocks, head_blocks, gap;   // blocks that somebody sees; those of the first keys; block of the window's first key
+};
+__device__ __forceinline__ uint32_t item_key0(const PromptItem& it, uint32_t j) { return (j < it.head_blocks ? j : it.gap + j - it.head_blocks) * 128; }
+__device__ __forceinline__ bool tile_sees(const PagedParams& p, const PromptItem& it, int t, uint32_t key0) {
+    return it.tokens[t] && (int32_t)key0 <= it.last[t] && (!p.a.window || key0 < p.a.sinks || (int64_t)key0 + 127 + p.a.window > it.first[t]);
+}
+// Whether a key of the block is hidden from some row between positions `first` and `last`.
+__device__ __forceinline__ bool partly_seen(const PagedParams& p, int32_t first, int32_t last, uint32_t key0) {
+    return (int64_t)key0 + 127 > first || (p.a.window && (int64_t)key0 + p.a.window <= last && key0 + 128 > p.a.sinks);
+}
+
+// Items in the order in which blocks of the grid take them: of every sequence and head the last tokens first (they have the most keys).
+__device__ __forceinline__ bool prompt_item(const PromptParams& prm, uint64_t index, PromptItem& it) {
+    const PagedParams& p = prm.p;
+    const uint32_t units = p.a.sequences * p.a.kv_heads, rest = (uint32_t)(index % units);
+    it.s = rest / p.a.kv_heads;
+    it.kvh = rest % p.a.kv_heads;
+    it.seq = paged_sequence(p, it.s);
+    const uint32_t pair = prm.pairs - 1 - (uint32_t)(index / units);
+    it.token0 = pair * 2 * prm.tokens;
+    if (it.token0 >= it.seq.count) return false;
+    const uint32_t left = it.seq.count - it.token0;
+    it.tokens[0] = min(left, prm.tokens);
+    it.tokens[1] = min(left - it.tokens[0], prm.tokens);
+    const int32_t base = (int32_t)it.seq.length - (int32_t)it.seq.count;
+    it.low = it.first[0] = base + (int32_t)it.token0;
+    it.last[0] = it.first[0] + (int32_t)it.tokens[0] - 1;
+    it.first[1] = it.last[0] + 1;
+    it.last[1] = it.last[0] + (int32_t)it.tokens[1];
+    it.high = it.last[1];
+    it.head_blocks = it.gap = it.blocks = 0;
+    if (it.high < 0) return true;
+    if (p.a.window && it.low >= (int32_t)p.a.window) {
+        it.gap = (uint32_t)(it.low + 1 - (int32_t)p.a.window) / 128;
+        it.head_blocks = min((min(p.a.sinks, (uint32_t)it.high + 1) + 127) / 128, it.gap);
+    }
+    it.blocks = it.head_blocks + (uint32_t)it.high / 128 - it.gap + 1;
+    return true;
+}
+
+template <int W>
+__global__ void __launch_bounds__(PP_THREADS, 1)
+paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ PromptParams prm) {
+    using S = PromptShape<W>;
+    constexpr uint32_t STAGES = S::STAGES, HALVES = W / 64;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* q_tiles = smem;                                   // [2]
+    uint8_t* k_ring = smem + 2 * S::TILE;                      // [STAGES]
+    uint8_t* v_ring = k_ring + STAGES * S::TILE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_ring + STAGES * S::TILE);
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8;       // a tile each
+    uint64_t *looked = bars + 10;                              // a tile each: its warps are through with an item's values
+    uint64_t *k_full = bars + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + STAGES);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* odd_seen = tmem_slot + 2;                        // [2 tiles][2]: last item of even or odd number in which something was found, and how many keys
+    uint32_t* odd_keys = odd_seen + 4;                         // [2 tiles][2][PP_ODD]
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagedParams& p = prm.p;
+    const uint64_t limit = prm.wait_limit_ns;
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full + t, 1);
+            mbar_init(q_empty + t, 1);
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+            mbar_init(o_full + t, 1);
+            mbar_init(looked + t, 4);
+            odd_seen[2 * t] = odd_seen[2 * t + 1] = 0;
+        }
+        for (uint32_t i = 0; i < STAGES; ++i) {
+            mbar_init(k_full + i, 1);
+            mbar_init(k_empty + i, 1);
+            mbar_init(v_full + i, 1);
+            mbar_init(v_empty + i, 1);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, PP_TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint64_t items = (uint64_t)p.a.sequences * p.a.kv_heads * prm.pairs;
+    PromptItem it;
+
+    if (warp == 0) {
+        // ---------------- copies ----------------
+        uint32_t blocks = 0, used[2] = {0, 0};       // key blocks so far; items so far that had rows in a tile
+        bool ok = true;
+        for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
+            if (!prompt_item(prm, index, it) || it.blocks == 0) continue;
+            const uint32_t boxes = 128 / prm.box;
+            for (uint32_t j = 0; ok && j < it.blocks; ++j, ++blocks) {
+                const uint32_t stage = blocks % STAGES, parity = ((blocks / STAGES) & 1) ^ 1;
+                const uint32_t key = item_key0(it, j) + lane * prm.box;
+                int32_t page = (int32_t)p.a.pool_pages, row = 0;          // outside: zeros
+                if (lane < boxes && (int32_t)key <= it.high &&
+                    (!p.a.window || key < p.a.sinks || (int64_t)key + prm.box - 1 + p.a.window > it.low)) {
+                    const uint32_t i = p.page.div(key), entry = p.a.table[(uint64_t)it.s * p.a.table_ld + i];
+                    row = (int32_t)(key - i * p.page.d);
+                    if (entry < p.a.pool_pages) page = (int32_t)entry;
+                    else report(p.a.d_status, DEV_BAD_PAGE);
+                }
+                ok = mbar_wait(k_empty + stage, parity, abort_flag, limit);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(k_full + stage, S::TILE);
+                __syncwarp();
+                if (lane < boxes)
+#pragma unroll
+                    for (uint32_t h = 0; h < HALVES; ++h)
+                        pp_load_4d(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_k, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
+                                   k_full + stage);
+                if (j == 0) {
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (!it.tokens[t]) continue;
+                        ok = used[t] == 0 || mbar_wait(q_empty + t, (used[t] - 1) & 1, abort_flag, limit);
+                        ++used[t];
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (ok && lane == 0) {
+                            mbar_expect_tx(q_full + t, HALVES * prm.tokens * p.per.d * 128);
+                            for (uint32_t h = 0; h < HALVES; ++h)
+                                pp_load_3d(smem_u32(q_tiles) + t * S::TILE + h * PP_HALF, &map_q, (int32_t)(h * 64), (int32_t)(it.kvh * p.per.d),
+                                           (int32_t)(it.seq.start + it.token0 + t * prm.tokens), q_full + t);
+                        }
+                    }
+                    if (!ok) break;
+                }
+                ok = mbar_wait(v_empty + stage, parity, abort_flag, limit);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(v_full + stage, S::TILE);
+                __syncwarp();
+                if (lane < boxes)
+#pragma unroll
+                    for (uint32_t h = 0; h < HALVES; ++h)
+                        pp_load_4d(smem_u32(v_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_v, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
+                                   v_full + stage);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+            uint32_t blocks = 0, used[2] = {0, 0}, seen[2] = {0, 0};     // key blocks; items; blocks of a tile so far
+            auto issue_s = [&](int t, uint32_t stage) {
+#pragma unroll
+                for (uint32_t h = 0; h < HALVES; ++h) {
+                    const uint64_t qdesc = make_kmajor_sw128_desc(smem_u32(q_tiles) + t * S::TILE + h * PP_HALF);
+                    const uint64_t kdesc = make_kmajor_sw128_desc(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF);
+#pragma unroll
+                    for (uint32_t kk = 0; kk < 4; ++kk) umma_bf16(tmem + t * 128, qdesc + kk * 2, kdesc + kk * 2, PP_IDESC_S, h != 0 || kk != 0);
+                }
+                umma_commit(s_full + t);
+            };
+            bool ok = true;
+            for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
+                if (!prompt_item(prm, index, it) || it.blocks == 0) continue;
+                // the last block that a tile sees: behind its scores the query tile may change, behind its product the output is complete
+                uint32_t last[2] = {0, 0}, first_product[2] = {1, 1};
+                for (uint32_t j = 0; j < it.blocks; ++j)
+                    for (int t = 0; t < 2; ++t)
+                        if (tile_sees(p, it, t, item_key0(it, j))) last[t] = j + 1;
+                for (int t = 0; t < 2 && ok; ++t)
+                    if (it.tokens[t]) {
+                        ok = mbar_wait(q_full + t, used[t] & 1, abort_flag, limit);
+                        ++used[t];
+                    }
+                if (!ok) break;
+                auto scores = [&](uint32_t j, int t) {
+                    if (tile_sees(p, it, t, item_key0(it, j))) issue_s(t, (blocks + j) % STAGES);
+                    // a tile without any block gives its query tile back with the item's first one
+                    if (it.tokens[t] && j + 1 == max(last[t], 1u)) umma_commit(q_empty + t);
+                };
+                auto wait_k = [&](uint32_t j) {
+                    const uint32_t b = blocks + j;
+                    if (!mbar_wait(k_full + b % STAGES, (b / STAGES) & 1, abort_flag, limit)) return false;
+                    tc_fence_after();
+                    return true;
+                };
+                if (!wait_k(0)) break;
+                scores(0, 0);
+                scores(0, 1);
+                umma_commit(k_empty + blocks % STAGES);
+                for (uint32_t j = 0; ok && j < it.blocks; ++j) {
+                    const uint32_t b = blocks + j, stage = b % STAGES, key0 = item_key0(it, j);
+                    const bool more = j + 1 < it.blocks;
+                    if ((more && !wait_k(j + 1)) || !mbar_wait(v_full + stage, (b / STAGES) & 1, abort_flag, limit)) {
+                        ok = false;
+                        break;
+                    }
+                    for (int t = 0; t < 2; ++t) {
+                        if (tile_sees(p, it, t, key0)) {
+                            if (!mbar_wait(p_full + t, seen[t] & 1, abort_flag, limit)) {
+                                ok = false;
+                                break;
+                            }
+                            ++seen[t];
+                            tc_fence_after();
+                            const uint32_t v_addr = smem_u32(v_ring) + stage * S::TILE;
+#pragma unroll
+                            for (uint32_t kk = 0; kk < 8; ++kk)
+                                pp_mma_ta(tmem + PP_O + t * W, tmem + t * 128 + kk * 8, make_mnmajor_sw128_desc(v_addr + kk * 2048, PP_HALF, 1024),
+                                          PP_IDESC_O<W>, kk != 0 || !first_product[t]);
+                            first_product[t] = 0;
+                            if (j + 1 == last[t]) umma_commit(o_full + t);
+                        }
+                        if (more) scores(j + 1, t);
+                    }
+                    if (!ok) break;
+                    umma_commit(v_empty + stage);
+                    if (more) umma_commit(k_empty + (b + 1) % STAGES);
+                }
+                blocks += it.blocks;
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- softmax ----------------
+        const int t = (int)(warp - 4) >> 2;
+        const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t s_addr = tmem + t * 128 + ((quarter * 32u) << 16), o_addr = tmem + PP_O + t * W + ((quarter * 32u) << 16);
+        const uint32_t my_token = p.per.div(row), my_head = row - my_token * p.per.d;
+        uint32_t blocks = 0, seen = 0, outputs = 0, number = 0;      // key blocks; blocks of the tile; outputs; items so far
+        bool ok = true;
+        // a warp gives up as a whole
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
+        for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
+            if (!prompt_item(prm, index, it)) continue;
+            if (!it.tokens[t]) {
+                blocks += it.blocks;
+                continue;
+            }
+            const int32_t at = it.first[t] + (int32_t)min(my_token, it.tokens[t] - 1);
+            ++number;
+            float m = -INFINITY, l = 0.0f;
+            bool any = false;
+            for (uint32_t j = 0; j < it.blocks; ++j) {
+                const uint32_t b = blocks + j, key0 = item_key0(it, j);
+                if (!tile_sees(p, it, t, key0)) continue;
+                any = true;
+                if (!wait(s_full + t, seen & 1)) { ok = false; break; }
+                ++seen;
+                tc_fence_after();
+                if (partly_seen(p, it.low, it.high, key0)) {
+                    // a row of values per thread.  Behind s_full: the products' thread has by then waited for the values of every earlier block, so that
+                    // the ring cannot be a whole turn behind, which a barrier's parity would not show
+                    if (!wait(v_full + b % STAGES, (b / STAGES) & 1)) { ok = false; break; }
+                    uint8_t* v_row = v_ring + (b % STAGES) * S::TILE + row * 128;
+                    bool found = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8 * HALVES; ++i) {
+                        uint4* x = reinterpret_cast<uint4*>(v_row + (i / 8) * PP_HALF + ((i + lane) & 7) * 16);
+                        uint4 v = *x;
+                        uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+                        bool here = false;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if ((e[k] & 0x7f80u) == 0x7f80u) { e[k] &= 0xffff0000u; here = true; }
+                            if ((e[k] & 0x7f800000u) == 0x7f800000u) { e[k] &= 0xffffu; here = true; }
+                        }
+                        if (here) *x = v;
+                        found |= here;
+                    }
+                    const uint32_t key = key0 + row;
+                    if (found && (int32_t)key <= it.high && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > it.low)) {
+                        const uint32_t slot = 2 * t + (number & 1);
+                        uint32_t now = *(volatile uint32_t*)(odd_seen + slot), then;
+                        do {
+                            then = now;
+                            now = atomicCAS(odd_seen + slot, then, then >> 8 != number ? number << 8 | 1u : min(then + 1, number << 8 | 255u));
+                        } while (now != then);
+                        const uint32_t place = then >> 8 != number ? 0u : then & 255u;
+                        if (place < PP_ODD) odd_keys[slot * PP_ODD + place] = key;
+                    }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                float v[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v + c * 32);
+                tmem_ld_wait();
+                if (partly_seen(p, it.first[t], it.last[t], key0)) {
+                    const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) {
+                        const int32_t key = (int32_t)key0 + i;
+                        if (key > at || (p.a.window && key < lowest && (uint32_t)key >= p.a.sinks)) v[i] = -INFINITY;
+                    }
+                }
+                float top4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 128; ++i) top4[i & 3] = fmaxf(top4[i & 3], v[i]);
+                top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                // `m` stays while weights do not grow past 2^8
+                float f = 1.0f;
+                if (m == -INFINITY) {
+                    m = top;
+                } else if ((top - m) * p.scale_log2 > 8.0f) {
+                    f = mx_ex2((m - top) * p.scale_log2);
+                    m = top;
+                }
+                if (__any_sync(0xffffffffu, f != 1.0f)) {
+                    l *= f;
+#pragma unroll
+                    for (int c = 0; c < W / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(o_addr + c * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= f;
+                        pp_st32(o_addr + c * 32, o);
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
+                float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = mx_ex2(fmaf(v[c * 32 + 2 * i], p.scale_log2, neg)), y = mx_ex2(fmaf(v[c * 32 + 2 * i + 1], p.scale_log2, neg));
+                        sum4[i & 3] += x + y;
+                        packed[i] = pack_bf16x2(x, y);
+                    }
+                    pp_st16(s_addr + c * 16, packed);
+                }
+                l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                pp_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t);
+            }
+            blocks += it.blocks;
+            if (!ok) break;
+            if (any) {
+                if (!wait(o_full + t, outputs & 1)) { ok = false; break; }
+                ++outputs;
+                tc_fence_after();
+            }
+            // whether the row sees something that must not be multiplied by 0 (a warp that is ahead writes to the other place)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(looked + t);
+            if (!wait(looked + t, (number - 1) & 1)) { ok = false; break; }
+            bool mine = my_token < it.tokens[t], odd = false;
+            const uint32_t slot = 2 * t + (number & 1), found = *(volatile uint32_t*)(odd_seen + slot);
+            if (found >> 8 == number) {
+                odd = (found & 255u) > PP_ODD;
+                for (uint32_t i = 0; i < min(found & 255u, PP_ODD); ++i) {
+                    const uint32_t key = odd_keys[slot * PP_ODD + i];
+                    odd |= (int32_t)key <= at && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > at);
+                }
+                odd &= mine;
+                mine &= !odd;
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            bf16* out = reinterpret_cast<bf16*>(p.a.out) + (uint64_t)(it.seq.start + it.token0 + t * prm.tokens + my_token) * p.a.out_ld +
+                        (uint64_t)(it.kvh * p.per.d + my_head) * p.a.vdim;
+#pragma unroll
+            for (int c = 0; c < W / 32; ++c) {
+                float o[32];
+                if (any) {
+                    tmem_ld32(o_addr + c * 32, o);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!mine || (uint32_t)(c * 32 + i * 8) >= p.a.vdim) continue;
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (l != 0.0f) {
+                        w.x = pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv);
+                        w.y = pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
+                        w.z = pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
+                        w.w = pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+                    }
+                    *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = w;
+                }
+            }
+            tc_fence_before();
+            for (uint32_t rows = __ballot_sync(0xffffffffu, odd); rows; rows &= rows - 1) {
+                const uint32_t r = quarter * 32 + __ffs(rows) - 1, token = p.per.div(r);
+                paged_row<bf16>(p, it.s, it.seq, it.seq.start + it.token0 + t * prm.tokens + token, it.kvh * p.per.d + r - token * p.per.d, lane);
+            }
+        }
+    }
+
+    // ---------------- teardown ----------------
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        // copies that are still on their way get time to land before the shared memory is somebody else's
+        const uint64_t start = global_timer_ns();
+        while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
+        if (threadIdx.x == 0) report(p.a.d_status, DEV_TIMEOUT);
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, PP_TMEM);
+    }
+}
+
+// ---- launch ------------------------------------------------------------------------------------------------------------------------
+static bool pp_map(CUtensorMap* map, const void* base, uint32_t rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+    cuuint64_t d[4], st[3];
+    cuuint32_t b[4], e[4] = {1, 1, 1, 1};
+    for (uint32_t i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i) st[i - 1] = strides[i - 1] * 2;
+    }
+    return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, st, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool paged_prompt_eligible(const PagedAttention& a, int dtype) {
+    const uint64_t strides = (uint64_t)a.dim | a.vdim | a.k_page | a.k_row | a.k_head | a.v_page | a.v_row | a.v_head | a.q_ld | a.out_ld | a.page_rows;
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
+    const uint64_t most = std::max({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head});
+    const uint64_t least = std::min({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head});
+    return dtype == TNSR_B200_BF16 && a.dim <= 128 && a.vdim <= 128 && strides % 8 == 0 && at % 16 == 0 && a.scale > 0.0f && a.heads / a.kv_heads <= 128 &&
+           least > 0 && most < (1ull << 38) && a.pool_pages < 0x7fffffffu && g_gemm_engine != 1 && encode_fn() != nullptr;
+}
+
+template <int W>
+static int launch_prompt_width(const PromptParams& prm, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
+    if (const int rc = allow_shared<paged_prompt_kernel<W>>(PromptShape<W>::BYTES, "paged_attention attribute")) return rc;
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const uint64_t items = (uint64_t)prm.p.a.sequences * prm.p.a.kv_heads * prm.pairs;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(items, sms > 0 ? sms : 148);
+    launch_kernel(paged_prompt_kernel<W>, dim3(grid), dim3(PP_THREADS), (size_t)PromptShape<W>::BYTES, stream, mq, mk, mv, prm);
+    return TNSR_B200_OK;
+}
+
+int launch_paged_prompt(const PagedParams& p, cudaStream_t stream) {
+    const PagedAttention& a = p.a;
+    PromptParams prm;
+    prm.p = p;
+    prm.tokens = 128 / p.per.d;
+    prm.pairs = ceil_div(a.chunk, 2 * prm.tokens);
+    prm.box = std::min(128u, a.page_rows & (0u - a.page_rows));
+    prm.wait_limit_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+    CUtensorMap mq, mk, mv;
+    const uint64_t q_dims[3] = {a.dim, a.heads, a.rows}, q_strides[2] = {a.dim, a.q_ld};
+    const uint32_t q_box[3] = {64, p.per.d, prm.tokens}, kv_box[4] = {64, 1, prm.box, 1};
+    const uint64_t k_dims[4] = {a.dim, a.kv_heads, a.page_rows, a.pool_pages}, v_dims[4] = {a.vdim, a.kv_heads, a.page_rows, a.pool_pages};
+    const uint64_t k_strides[3] = {a.k_head, a.k_row, a.k_page}, v_strides[3] = {a.v_head, a.v_row, a.v_page};
+    if (!pp_map(&mq, a.q, 3, q_dims, q_strides, q_box) || !pp_map(&mk, a.k_pool, 4, k_dims, k_strides, kv_box) ||
+        !pp_map(&mv, a.v_pool, 4, v_dims, v_strides, kv_box)) {
+        set_thread_error("paged_attention: tensor map encoding failed");
+        return TNSR_B200_ERR_CUDA;
+    }
+    return std::max(a.dim, a.vdim) <= 64 ? launch_prompt_width<64>(prm, mq, mk, mv, stream) : launch_prompt_width<128>(prm, mq, mk, mv, stream);
+}
+
+}  // namespace tb

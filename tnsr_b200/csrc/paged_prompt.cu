@@ -52,12 +52,24 @@ struct PromptParams {
     uint64_t wait_limit_ns;
 };
 
-__device__ __forceinline__ void pp_mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Matrix descriptors differ in their lower word only, by constants: one thread issues all products of the block, and what it computes
+// between them is time that the tensor cores wait.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void pp_mma(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t desc_high, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_low), "r"(b_low), "r"(desc_high), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
+        : "memory");
+}
+// The left operand in TMEM.
+__device__ __forceinline__ void pp_mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t desc_high, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_low), "r"(desc_high), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t* r) {
@@ -65,10 +77,24 @@ __device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t* r) {
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-__device__ __forceinline__ void pp_st32(uint32_t taddr, const float* v) {
-    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-    pp_st16(taddr, r);
-    pp_st16(taddr + 16, r + 16);
+// Behind this the values of earlier loads may be used (they pass through, so that no use of them moves ahead of the wait).
+__device__ __forceinline__ void pp_ld_wait(float (&v)[128]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 128; i += 16)
+        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]),
+                          "+f"(v[i + 8]), "+f"(v[i + 9]), "+f"(v[i + 10]), "+f"(v[i + 11]), "+f"(v[i + 12]), "+f"(v[i + 13]), "+f"(v[i + 14]), "+f"(v[i + 15]));
+}
+// 16 columns of a row, waited for.
+__device__ __forceinline__ void pp_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
 }
 __device__ __forceinline__ void pp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pp_load_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
@@ -80,22 +106,45 @@ __device__ __forceinline__ void pp_load_4d(uint32_t dst, const CUtensorMap* map,
                  ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// Two values at once.
+__device__ __forceinline__ uint64_t pp_pair(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ __forceinline__ void pp_split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t pp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pp_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+template <int N>
+__device__ __forceinline__ void pp_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void pp_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // Two tiles of a sequence and key/value head.
 struct PromptItem {
     PagedSequence seq;
     uint32_t s, kvh, token0;             // first token of the first tile
     uint32_t tokens[2];                  // of each tile
     int32_t first[2], last[2];           // positions of a tile's first and last token
-    int32_t low, high;                   // of the item's
+    int32_t from[2], whole[2];           // first key of the window of the tile's first row, and of its last
+    int32_t high;                        // position of the item's last token
     uint32_t blocks, head_blocks, gap;   // blocks that somebody sees; those of the first keys; block of the window's first key
 };
 __device__ __forceinline__ uint32_t item_key0(const PromptItem& it, uint32_t j) { return (j < it.head_blocks ? j : it.gap + j - it.head_blocks) * 128; }
+// Whether a row of the tile sees a key of the block; whether one of the rows of tiles t0 to t1 does not see one.
 __device__ __forceinline__ bool tile_sees(const PagedParams& p, const PromptItem& it, int t, uint32_t key0) {
-    return it.tokens[t] && (int32_t)key0 <= it.last[t] && (!p.a.window || key0 < p.a.sinks || (int64_t)key0 + 127 + p.a.window > it.first[t]);
+    return (int32_t)key0 <= it.last[t] && ((int32_t)key0 + 127 >= it.from[t] || key0 < p.a.sinks);
 }
-// Whether a key of the block is hidden from some row between positions `first` and `last`.
-__device__ __forceinline__ bool partly_seen(const PagedParams& p, int32_t first, int32_t last, uint32_t key0) {
-    return (int64_t)key0 + 127 > first || (p.a.window && (int64_t)key0 + p.a.window <= last && key0 + 128 > p.a.sinks);
+__device__ __forceinline__ bool partly_seen(const PagedParams& p, const PromptItem& it, int t0, int t1, uint32_t key0) {
+    return (int32_t)key0 + 127 > it.first[t0] || ((int32_t)key0 < it.whole[t1] && key0 + 128 > p.a.sinks);
 }
 
 // Items in the order in which blocks of the grid take them: of every sequence and head the last tokens first (they have the most keys).
@@ -112,19 +161,27 @@ __device__ __forceinline__ bool prompt_item(const PromptParams& prm, uint64_t in
     it.tokens[0] = min(left, prm.tokens);
     it.tokens[1] = min(left - it.tokens[0], prm.tokens);
     const int32_t base = (int32_t)it.seq.length - (int32_t)it.seq.count;
-    it.low = it.first[0] = base + (int32_t)it.token0;
+    it.first[0] = base + (int32_t)it.token0;
     it.last[0] = it.first[0] + (int32_t)it.tokens[0] - 1;
     it.first[1] = it.last[0] + 1;
-    it.last[1] = it.last[0] + (int32_t)it.tokens[1];
-    it.high = it.last[1];
+    it.last[1] = it.high = it.last[0] + (int32_t)it.tokens[1];
+    const int32_t window = (int32_t)min(p.a.window, 0x7fffffffu);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        it.from[t] = window && it.first[t] >= window ? it.first[t] - window + 1 : 0;
+        it.whole[t] = window && it.last[t] >= window ? it.last[t] - window + 1 : 0;
+    }
+    if (it.tokens[1] == 0) it.last[1] = -1;          // sees nothing
     it.head_blocks = it.gap = it.blocks = 0;
     if (it.high < 0) return true;
-    if (p.a.window && it.low >= (int32_t)p.a.window) {
-        it.gap = (uint32_t)(it.low + 1 - (int32_t)p.a.window) / 128;
-        it.head_blocks = min((min(p.a.sinks, (uint32_t)it.high + 1) + 127) / 128, it.gap);
-    }
+    it.gap = (uint32_t)it.from[0] / 128;
+    it.head_blocks = min((min(p.a.sinks, (uint32_t)it.high + 1) + 127) / 128, it.gap);
     it.blocks = it.head_blocks + (uint32_t)it.high / 128 - it.gap + 1;
     return true;
+}
+// Blocks up to the last one that a tile sees.
+__device__ __forceinline__ uint32_t tile_blocks(const PromptItem& it, int t) {
+    return it.last[t] < 0 ? 0u : it.head_blocks + (uint32_t)it.last[t] / 128 - it.gap + 1;
 }
 
 template <int W>
@@ -182,6 +239,25 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint64_t items = (uint64_t)p.a.sequences * p.a.kv_heads * prm.pairs;
     PromptItem it;
 
+    auto teardown = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        if (*abort_flag) {
+            // copies that are still on their way get time to land before the shared memory is somebody else's
+            const uint64_t start = global_timer_ns();
+            while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
+            if (threadIdx.x == 0) report(p.a.d_status, DEV_TIMEOUT);
+            __syncthreads();
+        }
+        if (warp == 1) {
+            tc_fence_after();
+            tmem_dealloc(tmem, PP_TMEM);
+        }
+    };
+    // The softmax warps' registers come from the others: 4 x 32 x 104 + 8 x 32 x 200 are no more than the 12 x 32 x 168 that the block starts with.
+    // The two kinds of warps do not meet again, or all would be held to the smaller number.
+    if (warp < 4) {
+        pp_fewer_registers<104>();
     if (warp == 0) {
         // ---------------- copies ----------------
         uint32_t blocks = 0, used[2] = {0, 0};       // key blocks so far; items so far that had rows in a tile
@@ -193,8 +269,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const uint32_t stage = blocks % STAGES, parity = ((blocks / STAGES) & 1) ^ 1;
                 const uint32_t key = item_key0(it, j) + lane * prm.box;
                 int32_t page = (int32_t)p.a.pool_pages, row = 0;          // outside: zeros
-                if (lane < boxes && (int32_t)key <= it.high &&
-                    (!p.a.window || key < p.a.sinks || (int64_t)key + prm.box - 1 + p.a.window > it.low)) {
+                if (lane < boxes && (int32_t)key <= it.high && (key < p.a.sinks || (int32_t)(key + prm.box) > it.from[0])) {
                     const uint32_t i = p.page.div(key), entry = p.a.table[(uint64_t)it.s * p.a.table_ld + i];
                     row = (int32_t)(key - i * p.page.d);
                     if (entry < p.a.pool_pages) page = (int32_t)entry;
@@ -241,78 +316,91 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         // ---------------- products ----------------
         if (lane == 0) {
             uint32_t blocks = 0, used[2] = {0, 0}, seen[2] = {0, 0};     // key blocks; items; blocks of a tile so far
+            const uint64_t kmajor = make_kmajor_sw128_desc(0), mnmajor = make_mnmajor_sw128_desc(0, PP_HALF, 1024);
+            const uint32_t k_high = (uint32_t)(kmajor >> 32), v_high = (uint32_t)(mnmajor >> 32);
+            const uint32_t q_low = (uint32_t)kmajor + (smem_u32(q_tiles) >> 4), k_low = (uint32_t)kmajor + (smem_u32(k_ring) >> 4),
+                           v_low = (uint32_t)mnmajor + (smem_u32(v_ring) >> 4);
             auto issue_s = [&](int t, uint32_t stage) {
+                const uint32_t a = q_low + t * (S::TILE >> 4), b = k_low + stage * (S::TILE >> 4);
 #pragma unroll
-                for (uint32_t h = 0; h < HALVES; ++h) {
-                    const uint64_t qdesc = make_kmajor_sw128_desc(smem_u32(q_tiles) + t * S::TILE + h * PP_HALF);
-                    const uint64_t kdesc = make_kmajor_sw128_desc(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF);
+                for (uint32_t h = 0; h < HALVES; ++h)
 #pragma unroll
-                    for (uint32_t kk = 0; kk < 4; ++kk) umma_bf16(tmem + t * 128, qdesc + kk * 2, kdesc + kk * 2, PP_IDESC_S, h != 0 || kk != 0);
-                }
+                    for (uint32_t kk = 0; kk < 4; ++kk) {
+                        if (h == 0 && kk == 0) pp_mma<false>(tmem + t * 128, a, b, k_high, PP_IDESC_S);
+                        else pp_mma<true>(tmem + t * 128, a + h * (PP_HALF >> 4) + kk * 2, b + h * (PP_HALF >> 4) + kk * 2, k_high, PP_IDESC_S);
+                    }
                 umma_commit(s_full + t);
             };
             bool ok = true;
             for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
                 if (!prompt_item(prm, index, it) || it.blocks == 0) continue;
-                // the last block that a tile sees: behind its scores the query tile may change, behind its product the output is complete
-                uint32_t last[2] = {0, 0}, first_product[2] = {1, 1};
-                for (uint32_t j = 0; j < it.blocks; ++j)
-                    for (int t = 0; t < 2; ++t)
-                        if (tile_sees(p, it, t, item_key0(it, j))) last[t] = j + 1;
+                // behind the scores of the last block that a tile sees its queries may change, behind its product the output is complete; a tile
+                // that sees nothing gives its queries back with the item's first block
+                const uint32_t last[2] = {tile_blocks(it, 0), tile_blocks(it, 1)};
+                uint32_t accumulate[2] = {0, 0};
                 for (int t = 0; t < 2 && ok; ++t)
                     if (it.tokens[t]) {
                         ok = mbar_wait(q_full + t, used[t] & 1, abort_flag, limit);
                         ++used[t];
                     }
                 if (!ok) break;
-                auto scores = [&](uint32_t j, int t) {
-                    if (tile_sees(p, it, t, item_key0(it, j))) issue_s(t, (blocks + j) % STAGES);
-                    // a tile without any block gives its query tile back with the item's first one
+                auto scores = [&](uint32_t j, int t, bool sees, uint32_t stage) {
+                    if (sees) issue_s(t, stage);
                     if (it.tokens[t] && j + 1 == max(last[t], 1u)) umma_commit(q_empty + t);
                 };
-                auto wait_k = [&](uint32_t j) {
-                    const uint32_t b = blocks + j;
-                    if (!mbar_wait(k_full + b % STAGES, (b / STAGES) & 1, abort_flag, limit)) return false;
-                    tc_fence_after();
-                    return true;
-                };
-                if (!wait_k(0)) break;
-                scores(0, 0);
-                scores(0, 1);
-                umma_commit(k_empty + blocks % STAGES);
-                for (uint32_t j = 0; ok && j < it.blocks; ++j) {
-                    const uint32_t b = blocks + j, stage = b % STAGES, key0 = item_key0(it, j);
+                uint32_t stage = blocks % STAGES, parity = (blocks / STAGES) & 1, key0 = item_key0(it, 0);
+                bool sees[2] = {tile_sees(p, it, 0, key0), tile_sees(p, it, 1, key0)};
+                if (!mbar_wait(k_full + stage, parity, abort_flag, limit)) break;
+                tc_fence_after();
+                scores(0, 0, sees[0], stage);
+                scores(0, 1, sees[1], stage);
+                umma_commit(k_empty + stage);
+                for (uint32_t j = 0; j < it.blocks; ++j) {
                     const bool more = j + 1 < it.blocks;
-                    if ((more && !wait_k(j + 1)) || !mbar_wait(v_full + stage, (b / STAGES) & 1, abort_flag, limit)) {
-                        ok = false;
-                        break;
+                    const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1, next_parity = next ? parity : parity ^ 1;
+                    bool then[2] = {false, false};
+                    if (more) {
+                        key0 = item_key0(it, j + 1);
+                        then[0] = tile_sees(p, it, 0, key0);
+                        then[1] = tile_sees(p, it, 1, key0);
+                        ok = mbar_wait(k_full + next, next_parity, abort_flag, limit);
                     }
+                    ok = ok && mbar_wait(v_full + stage, parity, abort_flag, limit);
+                    if (!ok) break;
+                    const uint32_t v = v_low + stage * (S::TILE >> 4);
+#pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (tile_sees(p, it, t, key0)) {
-                            if (!mbar_wait(p_full + t, seen[t] & 1, abort_flag, limit)) {
-                                ok = false;
-                                break;
-                            }
+                        if (sees[t]) {
+                            ok = ok && mbar_wait(p_full + t, seen[t] & 1, abort_flag, limit);
+                            if (!ok) break;
                             ++seen[t];
                             tc_fence_after();
-                            const uint32_t v_addr = smem_u32(v_ring) + stage * S::TILE;
+                            pp_mma_ta(tmem + PP_O + t * W, tmem + t * 128, v, v_high, PP_IDESC_O<W>, accumulate[t]);
 #pragma unroll
-                            for (uint32_t kk = 0; kk < 8; ++kk)
-                                pp_mma_ta(tmem + PP_O + t * W, tmem + t * 128 + kk * 8, make_mnmajor_sw128_desc(v_addr + kk * 2048, PP_HALF, 1024),
-                                          PP_IDESC_O<W>, kk != 0 || !first_product[t]);
-                            first_product[t] = 0;
+                            for (uint32_t kk = 1; kk < 8; ++kk)
+                                pp_mma_ta(tmem + PP_O + t * W, tmem + t * 128 + kk * 8, v + kk * 128, v_high, PP_IDESC_O<W>, 1);
+                            accumulate[t] = 1;
                             if (j + 1 == last[t]) umma_commit(o_full + t);
                         }
-                        if (more) scores(j + 1, t);
+                        if (more) scores(j + 1, t, then[t], next);
                     }
                     if (!ok) break;
                     umma_commit(v_empty + stage);
-                    if (more) umma_commit(k_empty + (b + 1) % STAGES);
+                    if (more) umma_commit(k_empty + next);
+                    sees[0] = then[0];
+                    sees[1] = then[1];
+                    stage = next;
+                    parity = next_parity;
                 }
                 blocks += it.blocks;
             }
         }
-    } else if (warp >= 4) {
+    }
+    teardown();
+    return;
+    }
+    pp_more_registers<200>();
+    {
         // ---------------- softmax ----------------
         const int t = (int)(warp - 4) >> 2;
         const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
@@ -330,6 +418,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             const int32_t at = it.first[t] + (int32_t)min(my_token, it.tokens[t] - 1);
             ++number;
+            const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
             float m = -INFINITY, l = 0.0f;
             bool any = false;
             for (uint32_t j = 0; j < it.blocks; ++j) {
@@ -339,7 +428,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (!wait(s_full + t, seen & 1)) { ok = false; break; }
                 ++seen;
                 tc_fence_after();
-                if (partly_seen(p, it.low, it.high, key0)) {
+                if (partly_seen(p, it, 0, it.tokens[1] ? 1 : 0, key0)) {
                     // a row of values per thread.  Behind s_full: the products' thread has by then waited for the values of every earlier block, so that
                     // the ring cannot be a whole turn behind, which a barrier's parity would not show
                     if (!wait(v_full + b % STAGES, (b / STAGES) & 1)) { ok = false; break; }
@@ -360,7 +449,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         found |= here;
                     }
                     const uint32_t key = key0 + row;
-                    if (found && (int32_t)key <= it.high && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > it.low)) {
+                    if (found && (int32_t)key <= it.high && ((int32_t)key >= it.from[0] || key < p.a.sinks)) {
                         const uint32_t slot = 2 * t + (number & 1);
                         uint32_t now = *(volatile uint32_t*)(odd_seen + slot), then;
                         do {
@@ -376,20 +465,20 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 float v[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v + c * 32);
-                tmem_ld_wait();
-                if (partly_seen(p, it.first[t], it.last[t], key0)) {
-                    const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
+                pp_ld_wait(v);
+                if (partly_seen(p, it, t, t, key0)) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i) {
                         const int32_t key = (int32_t)key0 + i;
-                        if (key > at || (p.a.window && key < lowest && (uint32_t)key >= p.a.sinks)) v[i] = -INFINITY;
+                        if (key > at || (key < lowest && (uint32_t)key >= p.a.sinks)) v[i] = -INFINITY;
                     }
                 }
                 float top4[4] = {m, -INFINITY, -INFINITY, -INFINITY};
-                float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 128; ++i) top4[i & 3] = fmaxf(top4[i & 3], v[i]);
-                top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                for (int i = 0; i < 128; i += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top4[k] = fmaxf(fmaxf(top4[k], v[i + 2 * k]), v[i + 2 * k + 1]);
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
                 // `m` stays while weights do not grow past 2^8
                 float f = 1.0f;
                 if (m == -INFINITY) {
@@ -401,29 +490,34 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (__any_sync(0xffffffffu, f != 1.0f)) {
                     l *= f;
 #pragma unroll
-                    for (int c = 0; c < W / 32; ++c) {
-                        float o[32];
-                        tmem_ld32(o_addr + c * 32, o);
-                        tmem_ld_wait();
+                    for (int c = 0; c < W / 16; ++c) {
+                        float o[16];
+                        pp_ld16(o_addr + c * 16, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] *= f;
-                        pp_st32(o_addr + c * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] *= f;
+                        pp_st16(o_addr + c * 16, reinterpret_cast<const uint32_t*>(o));
                     }
                 }
                 const float neg = m == -INFINITY ? 0.0f : -m * p.scale_log2;
-                float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t scale2 = pp_pair(p.scale_log2, p.scale_log2), neg2 = pp_pair(neg, neg);
+                uint64_t sums[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t packed[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = mx_ex2(fmaf(v[c * 32 + 2 * i], p.scale_log2, neg)), y = mx_ex2(fmaf(v[c * 32 + 2 * i + 1], p.scale_log2, neg));
-                        sum4[i & 3] += x + y;
+                        float x, y;
+                        pp_split(pp_fma2(pp_pair(v[c * 32 + 2 * i], v[c * 32 + 2 * i + 1]), scale2, neg2), x, y);
+                        x = mx_ex2(x);
+                        y = mx_ex2(y);
+                        sums[i & 1] = pp_add2(sums[i & 1], pp_pair(x, y));
                         packed[i] = pack_bf16x2(x, y);
                     }
                     pp_st16(s_addr + c * 16, packed);
                 }
-                l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                float sum_x, sum_y;
+                pp_split(pp_add2(sums[0], sums[1]), sum_x, sum_y);
+                l += sum_x + sum_y;
                 pp_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -455,15 +549,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             bf16* out = reinterpret_cast<bf16*>(p.a.out) + (uint64_t)(it.seq.start + it.token0 + t * prm.tokens + my_token) * p.a.out_ld +
                         (uint64_t)(it.kvh * p.per.d + my_head) * p.a.vdim;
 #pragma unroll
-            for (int c = 0; c < W / 32; ++c) {
-                float o[32];
-                if (any) {
-                    tmem_ld32(o_addr + c * 32, o);
-                    tmem_ld_wait();
-                }
+            for (int c = 0; c < W / 16; ++c) {
+                float o[16];
+                if (any) pp_ld16(o_addr + c * 16, o);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!mine || (uint32_t)(c * 32 + i * 8) >= p.a.vdim) continue;
+                for (int i = 0; i < 2; ++i) {
+                    if (!mine || (uint32_t)(c * 16 + i * 8) >= p.a.vdim) continue;
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
                     if (l != 0.0f) {
                         w.x = pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv);
@@ -471,7 +562,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         w.z = pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
                         w.w = pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
                     }
-                    *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = w;
+                    *reinterpret_cast<uint4*>(out + c * 16 + i * 8) = w;
                 }
             }
             tc_fence_before();
@@ -482,20 +573,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
     }
 
-    // ---------------- teardown ----------------
-    tc_fence_before();
-    __syncthreads();
-    if (*abort_flag) {
-        // copies that are still on their way get time to land before the shared memory is somebody else's
-        const uint64_t start = global_timer_ns();
-        while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
-        if (threadIdx.x == 0) report(p.a.d_status, DEV_TIMEOUT);
-        __syncthreads();
-    }
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem, PP_TMEM);
-    }
+    teardown();
 }
 
 // ---- launch ------------------------------------------------------------------------------------------------------------------------

@@ -433,20 +433,22 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     // the ring cannot be a whole turn behind, which a barrier's parity would not show
                     if (!wait(v_full + b % STAGES, (b / STAGES) & 1)) { ok = false; break; }
                     uint8_t* v_row = v_ring + (b % STAGES) * S::TILE + row * 128;
-                    bool found = false;
+                    // the order of the pieces by lane: neighbours read other banks.  An exponent of ones carries into the sign's place.
+                    uint32_t ones = 0;
 #pragma unroll
                     for (uint32_t i = 0; i < 8 * HALVES; ++i) {
-                        uint4* x = reinterpret_cast<uint4*>(v_row + (i / 8) * PP_HALF + ((i + lane) & 7) * 16);
-                        uint4 v = *x;
-                        uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-                        bool here = false;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if ((e[k] & 0x7f80u) == 0x7f80u) { e[k] &= 0xffff0000u; here = true; }
-                            if ((e[k] & 0x7f800000u) == 0x7f800000u) { e[k] &= 0xffffu; here = true; }
+                        const uint4 x = *reinterpret_cast<const uint4*>(v_row + (i / 8) * PP_HALF + ((i + lane) & 7) * 16);
+                        ones |= ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
+                                ((x.w & 0x7f807f80u) + 0x00800080u);
+                    }
+                    const bool found = ones & 0x80008000u;
+                    if (found) {
+#pragma unroll 1
+                        for (uint32_t i = 0; i < 32 * HALVES; ++i) {
+                            uint32_t* x = reinterpret_cast<uint32_t*>(v_row + (i / 32) * PP_HALF) + i % 32;
+                            const uint32_t v = *x, odd = ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                            if (odd) *x = v & ~((odd & 0x8000u ? 0xffffu : 0u) | (odd & 0x80000000u ? 0xffff0000u : 0u));
                         }
-                        if (here) *x = v;
-                        found |= here;
                     }
                     const uint32_t key = key0 + row;
                     if (found && (int32_t)key <= it.high && ((int32_t)key >= it.from[0] || key < p.a.sinks)) {
@@ -467,10 +469,20 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v + c * 32);
                 pp_ld_wait(v);
                 if (partly_seen(p, it, t, t, key0)) {
+                    // one edge or the other; both and the first keys only where they meet in a block
+                    const int32_t high = at - (int32_t)key0, low = lowest - (int32_t)key0, head = (int32_t)min(p.a.sinks, 0x7fffffffu) - (int32_t)key0;
+                    if ((int32_t)key0 >= it.whole[t]) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) {
-                        const int32_t key = (int32_t)key0 + i;
-                        if (key > at || (key < lowest && (uint32_t)key >= p.a.sinks)) v[i] = -INFINITY;
+                        for (int i = 0; i < 128; ++i)
+                            if (i > high) v[i] = -INFINITY;
+                    } else if ((int32_t)key0 + 127 <= it.first[t] && head <= 0) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i < low) v[i] = -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i > high || (i < low && i >= head)) v[i] = -INFINITY;
                     }
                 }
                 float top4[4] = {m, -INFINITY, -INFINITY, -INFINITY};

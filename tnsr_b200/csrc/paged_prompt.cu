@@ -254,10 +254,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tmem_dealloc(tmem, PP_TMEM);
         }
     };
-    // The softmax warps' registers come from the others: 4 x 32 x 104 + 8 x 32 x 200 are no more than the 12 x 32 x 168 that the block starts with.
+    // The softmax warps' registers come from the others: 4 x 32 x 104 + 8 x 32 x 200 (or 88 and 208) are no more than the 12 x 32 x 168 that the block starts with.
     // The two kinds of warps do not meet again, or all would be held to the smaller number.
     if (warp < 4) {
-        pp_fewer_registers<104>();
+        pp_fewer_registers<W == 64 ? 88 : 104>();
     if (warp == 0) {
         // ---------------- copies ----------------
         uint32_t blocks = 0, used[2] = {0, 0};       // key blocks so far; items so far that had rows in a tile
@@ -399,7 +399,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     teardown();
     return;
     }
-    pp_more_registers<200>();
+    pp_more_registers<W == 64 ? 208 : 200>();
     {
         // ---------------- softmax ----------------
         const int t = (int)(warp - 4) >> 2;

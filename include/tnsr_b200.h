@@ -812,7 +812,7 @@ typedef struct tnsr_b200_beam_select_args {
     float* next_scores;
     uint32_t *tokens, *parents;
     uint8_t* next_finished;       /* may be NULL */
-    void* workspace;              /* tnsr_b200_beam_select_workspace(); its contents do not matter */
+    void* workspace;              /* tnsr_b200_beam_select_workspace() bytes */
     uint64_t workspace_bytes, logits_ld;
     uint32_t groups, beams, vocab, keep, end_token;
     int32_t dtype;

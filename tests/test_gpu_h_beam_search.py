@@ -26,7 +26,7 @@ def select(logits, scores, finished, groups, beams, keep, end, ld=None, work=Non
     out = [torch.full((groups, keep), -7, dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32)]
     done = torch.full((groups, keep), 7, dtype=torch.uint8, device="cuda")
     if work is None:
-        work = scratch(lib().tnsr_b200_beam_select_workspace(groups, beams, vocab, keep)).fill_(0xa5)
+        work = scratch(lib().tnsr_b200_beam_select_workspace(groups, beams, vocab, keep))
     _KEEP.extend([room, scores, finished, work, done, *out])
     args = _native.BeamSelectArgs(logits=rows.data_ptr(), scores=scores.data_ptr(), finished=None if finished is None else finished.data_ptr(),
                                   next_scores=out[0].data_ptr(), tokens=out[1].data_ptr(), parents=out[2].data_ptr(), next_finished=done.data_ptr(),

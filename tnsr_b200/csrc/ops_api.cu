@@ -361,7 +361,7 @@ int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, void* stream) 
         return bad("beam_select: null pointer");
     if (!two_types(args->dtype)) return bad("beam_select: dtype must be f32 or bf16");
     if (args->beams == 0 || args->beams > BEAM_MAX || args->keep == 0 || args->keep > BEAM_MAX_KEEP || args->vocab == 0 || args->vocab > BEAM_MAX_VOCAB ||
-        args->keep > (uint64_t)args->beams * args->vocab || args->logits_ld < args->vocab || (uint64_t)args->groups * args->beams > 0x7fffffffu)
+        args->keep > (uint64_t)args->beams * args->vocab || args->logits_ld < args->vocab || (uint64_t)args->groups * args->beams > 0x3ffffffu)
         return bad("beam_select: 1 to 32 beams, 1 to 64 candidates (no more than there are), a vocabulary of 1 to 2^26 that fits its rows");
     if (args->workspace_bytes < beam_select_workspace_bytes(args->groups, args->beams, args->vocab, args->keep) || !aligned16(args->workspace))
         return bad("beam_select: workspace smaller than tnsr_b200_beam_select_workspace() asks for, or not 16-byte aligned");

@@ -18,12 +18,14 @@
 #include <cmath>
 
 #include "beam.cuh"
+#include "tc_common.cuh"
 
 namespace tb {
 
 constexpr uint32_t BS_THREADS = 256, BS_WARPS = BS_THREADS / 32;
 constexpr uint32_t BS_RUNS = 32;              // runs of a row at the most
-constexpr uint32_t BS_BLOCKS = 592;           // four of an SM
+constexpr uint32_t BS_BLOCKS = 296;           // two of an SM
+constexpr uint32_t BS_LEAST_RUN = 2048;       // values of a run at the least, if the row has them
 constexpr uint32_t BS_GATHER = 4096;         // room for what is gathered: more than BEAM_MAX_KEEP * (32 + 1)
 
 // Order of floats as of integers; -0 is 0.
@@ -76,27 +78,16 @@ static MergeShape merge_shape(uint32_t beams, uint32_t runs, uint32_t keep) {
     m.bounds = ceil_div(keep, m.place + 1);
     return m;
 }
-// What can be at or above the bound: `bounds` lists with all of theirs, the others with less than `place + 1`; of several bounds the one that lets the fewest in.
-static uint32_t merge_room(const MergeShape& m, uint32_t keep) {
-    auto room = [&](uint32_t place) {
-        const uint32_t nth = ceil_div(keep, place + 1);
-        return nth * keep + (m.lists - nth) * place;
-    };
-    if (m.lists > BS_FEW_LISTS) return room(m.place);
-    uint32_t least = 0xffffffffu;
-    for (uint32_t w = 0; w < BS_WARPS; ++w) {
-        const uint32_t place = (1u << w) - 1;
-        if (place < keep && m.lists * (place + 1) >= keep) least = std::min(least, room(place));
-    }
-    return least;
-}
+// What can be at or above the bound: `bounds` lists with all of theirs, the others with less than `place + 1`.
+static uint32_t merge_room(const MergeShape& m, uint32_t keep) { return m.bounds * keep + (m.lists - m.bounds) * m.place; }
 
 // By one block.  `space`: [lists] at the place of the bound, what is gathered, and (`staged`) the lists.
 __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, const MergeShape& shape, uint32_t room, bool staged, const BeamRun* parts,
                            const uint64_t* lists, BeamCandidate* space) {
     __shared__ double offset[BEAM_MAX];           // of a beam's logits; NaN: all of its candidates are -inf
-    __shared__ uint8_t ended[BEAM_MAX];
-    __shared__ BeamCandidate bound, bounds[BS_WARPS];
+    __shared__ uint8_t ended[BEAM_MAX], was[BEAM_MAX];
+    __shared__ BeamCandidate bound;
+    __shared__ uint32_t places[BS_WARPS];
     __shared__ uint32_t count;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = group * b.beams;
     // what the sums do not wait for first
@@ -118,6 +109,7 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane == 0) {
+            was[beam] = over;
             ended[beam] = over && b.end_token < b.vocab && isfinite(c);
             const double total = top + log(sum);
             offset[beam] = !over && isfinite(total) && isfinite(c) ? (double)c - total : nan("");
@@ -142,45 +134,48 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
         if (key == 0) return {0, 0};
         return bs_candidate(o + bs_value((uint32_t)(key >> 32)), beam, (uint32_t)(key >> 32), ~(uint32_t)key);
     };
-    // The bound.  If the q-th largest of the lists' entries at place p has (p + 1) q >= keep, so many entries are at or above it.  Few lists: a warp each for
-    // places 0, 1, 3, 7, ..., and the largest of what they find (heads alone let all of a good beam's lists in where the beams lie far apart).
+    // The bound.  If the q-th largest of the lists' entries at place p has (p + 1) q >= keep, so many entries are at or above it.  Few lists: by scores rounded
+    // down to f32, a warp each for places 0, 1, 3, 7, ..., and the largest of what they find (heads alone let all of a good beam's lists in where the beams
+    // lie far apart).  Many lists, or too many equal scores: by one place, exactly.
+    auto single = [&](const BeamCandidate& c) -> uint32_t {      // 0: no candidate
+        if (!c.score) return 0u;
+        const uint64_t bits = c.score >> 63 ? c.score & 0x7fffffffffffffffull : ~c.score;
+        return bs_ordered(__double2float_rd(__longlong_as_double((long long)bits)));
+    };
+    BeamCandidate* gathered = space + shape.lists;
+    uint32_t n = room + 1;
     if (shape.lists <= BS_FEW_LISTS) {
-        const uint32_t place = (1u << warp) - 1;
-        const bool there = place < b.keep && (uint64_t)shape.lists * (place + 1) >= b.keep;
-        const uint32_t nth = (b.keep + place) / (place + 1);
-        if (tid < BS_WARPS) bounds[tid] = {0, 0};
-        __syncthreads();
-        if (there) {
-            BeamCandidate mine[BS_FEW_LISTS / 32];
-            uint32_t rank[BS_FEW_LISTS / 32] = {};
+        const uint32_t place = (1u << warp) - 1, nth = (b.keep + place) / (place + 1);
+        uint32_t found = 0;
+        if (place < b.keep && (uint64_t)shape.lists * (place + 1) >= b.keep) {
+            const uint32_t key[2] = {lane < shape.lists ? single(entry(lane, place)) : 0u, lane + 32 < shape.lists ? single(entry(lane + 32, place)) : 0u};
+            uint32_t rank[2] = {0, 0};
 #pragma unroll
-            for (int k = 0; k < (int)BS_FEW_LISTS / 32; ++k) mine[k] = k * 32 + lane < shape.lists ? entry(k * 32 + lane, place) : BeamCandidate{0, 0};
-#pragma unroll
-            for (int k = 0; k < (int)BS_FEW_LISTS / 32; ++k) {
-                if (k * 32 >= shape.lists) break;
-#pragma unroll 8
-                for (int i = 0; i < 32; ++i) {
-                    BeamCandidate other;
-                    other.score = __shfl_sync(0xffffffffu, mine[k].score, i);
-                    other.rest = __shfl_sync(0xffffffffu, mine[k].rest, i);
-#pragma unroll
-                    for (int m = 0; m < (int)BS_FEW_LISTS / 32; ++m) rank[m] += bs_better(other, mine[m]);
-                }
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t x = __shfl_sync(0xffffffffu, key[0], i), y = __shfl_sync(0xffffffffu, key[1], i);
+                rank[0] += (x > key[0]) + ((x == key[0]) & (i < lane)) + (y > key[0]);
+                rank[1] += (x >= key[1]) + (y > key[1]) + ((y == key[1]) & (i < lane));
             }
-            // only what is missing is equal, and below everything
+            found = __reduce_max_sync(0xffffffffu, rank[0] == nth - 1 ? key[0] : rank[1] == nth - 1 ? key[1] : 0u);
+        }
+        if (lane == 0) places[warp] = found;
+        __syncthreads();
+        uint32_t low = places[0];
 #pragma unroll
-            for (int k = 0; k < (int)BS_FEW_LISTS / 32; ++k)
-                if (rank[k] == nth - 1 && mine[k].score) bounds[warp] = mine[k];
+        for (int w = 1; w < (int)BS_WARPS; ++w) low = max(low, places[w]);
+        for (uint32_t x = tid; x < shape.lists * b.keep; x += BS_THREADS) {
+            const BeamCandidate c = entry(x / b.keep, x % b.keep);
+            if (c.score && single(c) >= low) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < room) gathered[at] = c;
+            }
         }
         __syncthreads();
-        if (tid == 0) {
-            BeamCandidate best = bounds[0];
-            for (uint32_t w = 1; w < BS_WARPS; ++w)
-                if (bs_better(bounds[w], best)) best = bounds[w];
-            bound = best;
-        }
+        n = count;
         __syncthreads();
-    } else {
+    }
+    if (n > room) {
+        if (tid == 0) count = 0;
         for (uint32_t l = tid; l < shape.lists; l += BS_THREADS) space[l] = entry(l, shape.place);
         __syncthreads();
         for (uint32_t l = tid; l < shape.lists; l += BS_THREADS) {
@@ -191,37 +186,38 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
             if (rank == shape.bounds - 1) bound = c;
         }
         __syncthreads();
+        const BeamCandidate low = bound;
+        for (uint32_t x = tid; x < shape.lists * b.keep; x += BS_THREADS) {
+            const BeamCandidate c = entry(x / b.keep, x % b.keep);
+            if (c.score && !bs_better(low, c)) gathered[atomicAdd(&count, 1u)] = c;
+        }
+        __syncthreads();
+        n = count;
     }
-    const BeamCandidate low = bound;
-    BeamCandidate* gathered = space + shape.lists;
-    for (uint32_t x = tid; x < shape.lists * b.keep; x += BS_THREADS) {
-        const BeamCandidate c = entry(x / b.keep, x % b.keep);
-        if (c.score && !bs_better(low, c)) gathered[atomicAdd(&count, 1u)] = c;
-    }
-    __syncthreads();
-    const uint32_t n = count;
-    for (uint32_t x = tid; x < n; x += BS_THREADS) {
-        const BeamCandidate c = gathered[x];
+    // ranks, eight threads a candidate
+    for (uint32_t x0 = 0; x0 < n; x0 += BS_THREADS / 8) {
+        const uint32_t x = x0 + tid / 8;
+        const BeamCandidate c = gathered[min(x, n - 1)];
         uint32_t rank = 0;
-        for (uint32_t i0 = 0; i0 < n && rank < b.keep; i0 += 8)
+        for (uint32_t i = tid % 8; i < n; i += 8) rank += bs_better(gathered[i], c);
 #pragma unroll
-            for (uint32_t i = i0; i < i0 + 8; ++i) rank += i < n && bs_better(gathered[min(i, n - 1)], c);
-        if (rank >= b.keep) continue;
+        for (int d = 1; d < 8; d *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+        if (tid % 8 || x >= n || rank >= b.keep) continue;
         const uint32_t beam = 63 - (uint32_t)(c.rest >> 58), token = BEAM_MAX_VOCAB - 1 - (uint32_t)(c.rest & (BEAM_MAX_VOCAB - 1));
         const uint64_t at = (uint64_t)group * b.keep + rank, bits = c.score >> 63 ? c.score & 0x7fffffffffffffffull : ~c.score;
         b.next_scores[at] = (float)__longlong_as_double((long long)bits);
         b.tokens[at] = token;
         b.parents[at] = first + beam;
-        if (b.next_finished) b.next_finished[at] = (b.finished && b.finished[first + beam]) || token == b.end_token;
+        if (b.next_finished) b.next_finished[at] = was[beam] || token == b.end_token;
     }
 }
 
 __global__ void __launch_bounds__(BS_THREADS) beam_merge_kernel(BeamSelect b, uint32_t runs, MergeShape shape, uint32_t room, bool staged, const BeamRun* parts,
                                                                 const uint64_t* lists) {
-    extern __shared__ BeamCandidate merge_space[];
+    extern __shared__ __align__(16) uint8_t space[];
     pdl_wait();
     pdl_trigger();
-    beam_merge(b, blockIdx.x, runs, shape, room, staged, parts, lists, merge_space);
+    beam_merge(b, blockIdx.x, runs, shape, room, staged, parts, lists, reinterpret_cast<BeamCandidate*>(space));
 }
 
 // Descending order over the lanes.
@@ -240,12 +236,15 @@ __device__ __forceinline__ float bs_sort_warp(float v, uint32_t lane) {
 __device__ __forceinline__ void bs_rank(uint64_t* gathered, uint32_t n, uint32_t keep, uint64_t* best) {
     const uint32_t tid = threadIdx.x;
     if (n <= 2 * BS_THREADS) {
-        for (uint32_t x = tid; x < n; x += BS_THREADS) {
-            const uint64_t mine = gathered[x];
+        // eight threads a key
+        for (uint32_t x0 = 0; x0 < n; x0 += BS_THREADS / 8) {
+            const uint32_t x = x0 + tid / 8;
+            const uint64_t mine = gathered[min(x, n - 1)];
             uint32_t rank = 0;
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; ++i) rank += gathered[i] > mine;
-            if (rank < keep) best[rank] = mine;
+            for (uint32_t i = tid % 8; i < n; i += 8) rank += gathered[i] > mine;
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+            if (tid % 8 == 0 && x < n && rank < keep) best[rank] = mine;
         }
     } else {                     // something unusual: by sorting
         uint32_t size = 2 * BS_THREADS;
@@ -306,73 +305,106 @@ __device__ uint32_t bs_select_exactly(const T* row, uint32_t first, uint32_t end
     return kept;
 }
 
-// `PER` values a thread at a time.  VEC: 16-byte loads.
-// Per value: a load, a maximum, a multiplication-addition, an exponential and an addition.  The few threads with a value at or above the bound have their values
-// read once more, from L2.
-template <typename T, int PER, bool VEC>
+// A piece of a run is 16 values a thread; three of them are on their way to shared memory by bulk copies.
+constexpr uint32_t BS_PIECE = 16 * BS_THREADS, BS_STAGES = 3;
+template <typename T>
+struct BeamStage {
+    static constexpr uint32_t BYTES = BS_PIECE * sizeof(T) + 16;
+    static constexpr uint32_t SPACE = BS_STAGES * BYTES > BS_GATHER * 8 ? BS_STAGES * BYTES : BS_GATHER * 8;
+};
+
+// Per value: a load from shared memory, a maximum, a multiplication-addition, an exponential and an addition.  The few threads with a value at or above the bound
+// have their values read once more, from L2.  Rows start anywhere: a copy takes the 16-byte units that its values lie in, and so what is beside them in the
+// array; what would lie outside the array is read value by value.
+template <typename T>
 __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, uint32_t run, uint32_t row_runs, BeamRun* runs, uint64_t* lists, MergeShape shape, uint32_t room,
-                                                                  bool staged, uint32_t* tickets) {
-    constexpr int W = VEC ? 16 / sizeof(T) : 1;
+                                                                  bool staged, uint32_t* tickets, uint64_t wait_limit_ns) {
+    constexpr int W = 4 / sizeof(T);                     // neighbours that a thread has together
     constexpr int TOPS = BEAM_MAX_KEEP / BS_WARPS;       // of a warp, for the bound
-    __shared__ __align__(16) uint64_t gathered[BS_GATHER];
-    __shared__ uint64_t best[BEAM_MAX_KEEP], tops[BS_THREADS], exact_bound;
+    extern __shared__ __align__(16) uint8_t space[];     // BeamStage<T>::SPACE
+    __shared__ uint64_t best[BEAM_MAX_KEEP], tops[BS_THREADS], exact_bound, full[BS_STAGES];
     __shared__ float warp_tops[BS_WARPS][TOPS];
     __shared__ double sums[BS_WARPS];
-    __shared__ uint32_t count;
+    __shared__ uint32_t count, threads;
+    __shared__ uint8_t listed[BS_THREADS];
+    __shared__ int gave_up;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < BS_STAGES; ++i) mbar_init(full + i, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
     // runs of a row, rows of a group behind one another: a group is complete before the last blocks of the launch begin
     const uint32_t row_number = blockIdx.x / row_runs, keep = b.keep;
     const T* row = reinterpret_cast<const T*>(b.logits) + (uint64_t)row_number * b.logits_ld;
-    const uint32_t first = blockIdx.x % row_runs * run, end = min(b.vocab, first + run);
+    const uint32_t first = blockIdx.x % row_runs * run, end = min(b.vocab, first + run), pieces = (end - first + BS_PIECE - 1) / BS_PIECE;
+    // the array in whole units
+    const uintptr_t inside = ((uintptr_t)b.logits + 15) & ~(uintptr_t)15,
+                    outside = (uintptr_t)(reinterpret_cast<const T*>(b.logits) + ((uint64_t)b.groups * b.beams - 1) * b.logits_ld + b.vocab) & ~(uintptr_t)15;
+    const uint32_t skew = (uint32_t)((uintptr_t)(row + first) & 15);      // bytes before a piece's first value in its first unit: pieces are whole units
+    auto fetch = [&](uint32_t i) {                                        // by one thread
+        const uintptr_t begin = (uintptr_t)(row + first + i * BS_PIECE) - skew, stop = (uintptr_t)(row + min(end, first + (i + 1) * BS_PIECE));
+        const uintptr_t from = max(begin, inside), to = min((stop + 15) & ~(uintptr_t)15, outside);
+        const uint32_t stage = i % BS_STAGES, bytes = to > from ? (uint32_t)(to - from) : 0u;
+        mbar_expect_tx(full + stage, bytes);
+        if (bytes)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(smem_u32(space + stage * BeamStage<T>::BYTES) + (uint32_t)(from - begin)), "l"(from), "r"(bytes), "r"(smem_u32(full + stage))
+                         : "memory");
+    };
+    if (tid == 0)
+        for (uint32_t i = 0; i < min(pieces, BS_STAGES); ++i) fetch(i);
 
     // The thread's largest value and its sum of exponentials.  A term is 2^(x L + shift) with L the float nearest to log2(e): the base of the sum is what the
     // rounded shift stands for and not the maximum it was made from, or all terms would be off by the same factor.
     float mine = -INFINITY, shift = 0.0f;
     double sum = 0.0;
-    for (uint32_t base = first; base < end; base += PER * BS_THREADS) {
+    for (uint32_t i = 0; i < pieces; ++i) {
+        const uint32_t stage = i % BS_STAGES, base = first + i * BS_PIECE, here = min(end - base, BS_PIECE);
+        if (!mbar_wait(full + stage, (i / BS_STAGES) & 1, &gave_up, wait_limit_ns)) sum = nan("");      // the row does not count then
         // value j * W + e of the thread is number (j * BS_THREADS + tid) * W + e of the piece; what is not there is -inf
-        float v[PER];
-        const uint32_t here = min(end - base, (uint32_t)PER * BS_THREADS), whole = here / (BS_THREADS * W);
-        const T* src = row + base + tid * W;
-        auto load = [&](int j, bool check) {
-            if (VEC && !check) {
-                const uint4 u = *reinterpret_cast<const uint4*>(src + j * BS_THREADS * W);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        float v[16];
+        const uint8_t* src = space + stage * BeamStage<T>::BYTES + skew;
+        const uintptr_t at = (uintptr_t)(row + base);
+        if (here == BS_PIECE && at >= inside && at + BS_PIECE * sizeof(T) <= outside) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (sizeof(T) == 4) {
-                        v[j * W + e] = __uint_as_float(w[e]);
-                    } else {
-                        const float2 f = bf16x2_to_f32(w[e]);
-                        v[j * W + 2 * e] = f.x;
-                        v[j * W + (W > 1 ? 2 * e + 1 : 0)] = f.y;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e)
-                    v[j * W + e] = !check || (j * BS_THREADS + tid) * W + e < here ? to_f32(src[j * BS_THREADS * W + e]) : -INFINITY;
-            }
-        };
-        if (whole == PER / W) {
-#pragma unroll
-            for (int j = 0; j < PER / W; ++j) load(j, false);
-        } else {
-#pragma unroll
-            for (int j = 0; j < PER / W; ++j) {
-                if (j * BS_THREADS * W < here) {
-                    load(j, true);
+            for (int j = 0; j < 16 / W; ++j) {
+                const uint8_t* x = src + (j * BS_THREADS + tid) * 4;
+                if (W == 1) {
+                    v[j] = *reinterpret_cast<const float*>(x);
+                } else if (skew % 4 == 0) {
+                    const float2 f = bf16x2_to_f32(*reinterpret_cast<const uint32_t*>(x));
+                    v[j * W] = f.x;
+                    v[j * W + W - 1] = f.y;
                 } else {
 #pragma unroll
-                    for (int e = 0; e < W; ++e) v[j * W + e] = -INFINITY;
+                    for (int e = 0; e < W; ++e) v[j * W + e] = to_f32(reinterpret_cast<const T*>(x)[e]);
                 }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint32_t k = (j / W * BS_THREADS + tid) * W + j % W;
+                v[j] = -INFINITY;
+                if (k < here) {
+                    const bool copied = (at + k * sizeof(T)) >= inside && (at + (k + 1) * sizeof(T)) <= outside;
+                    v[j] = to_f32(copied ? reinterpret_cast<const T*>(src)[k] : row[base + k]);
+                }
+            }
+        }
+        if (pieces > BS_STAGES) {
+            __syncthreads();             // the stage may be overwritten
+            if (tid == 0 && i + BS_STAGES < pieces) {
+                fence_proxy_async_smem();
+                fetch(i + BS_STAGES);
             }
         }
         float largest = v[0];
 #pragma unroll
-        for (int i = 1; i < PER; ++i) largest = fmaxf(largest, v[i]);
+        for (int j = 1; j < 16; ++j) largest = fmaxf(largest, v[j]);
         if (largest > mine) {
             const float now = -largest * BS_LOG2E;
             if (mine != -INFINITY) sum *= bs_ex2(now - shift);
@@ -381,9 +413,14 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
         }
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < PER; ++i) part[i & 3] += bs_ex2(fmaf(v[i], BS_LOG2E, shift));
+        for (int j = 0; j < 16; ++j) part[j & 3] += bs_ex2(fmaf(v[j], BS_LOG2E, shift));
         sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
     }
+    if (gave_up) {                       // copies that are still on their way get time to land
+        const uint64_t start = global_timer_ns();
+        while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
+    }
+    uint64_t* gathered = reinterpret_cast<uint64_t*>(space);        // behind the barrier below
     // the largest of the warp's threads, one after the other (equal ones count once: the bound may be lower then, and is one still)
     {
         uint32_t left = bs_ordered(mine);
@@ -396,7 +433,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
             if (left == largest) left = 0x007fffffu;      // -inf
         }
     }
-    if (tid == 0) count = 0;
+    if (tid == 0) count = threads = 0;
     __syncthreads();
     // The bound: the keep-th largest of the four largest of every warp's threads, or (more than 32) the smallest of the warps' eighth ones.
     float low, top;
@@ -413,28 +450,37 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
             top = fmaxf(top, warp_tops[w][0]);
         }
     }
-    // Threads with a value at or above the bound: the warp reads such a thread's values again, a value a lane.  Where the bound is -inf, which is also what
-    // stands for values behind the end, and where equal values let too many in, all is done exactly.
-    if (low != -INFINITY)
-        for (uint32_t who = __ballot_sync(0xffffffffu, mine >= low); who; who &= who - 1) {
-            const uint32_t other = tid - lane + __ffs(who) - 1;
-#pragma unroll 4
-            for (uint32_t i = lane;; i += 32) {
-                const uint32_t index = first + ((i / W) * BS_THREADS + other) * W + i % W;
-                if (!__any_sync(0xffffffffu, index < end)) break;
-                const float x = index < end ? to_f32(row[index]) : -INFINITY;
-                if (x >= low) {
-                    const uint32_t at = atomicAdd(&count, 1u);
-                    if (at < 2 * BS_THREADS) gathered[at] = bs_key(x, index);
-                }
-            }
-        }
+    // Threads with a value at or above the bound, a list of which is divided among the warps, have their values read again, a value a lane, four (of two threads
+    // eight) on their way at a time.  Where the bound is -inf, which is also what stands for values behind the end, and where equal values let too many in, all
+    // is done exactly.
+    if (mine >= low && low != -INFINITY) listed[atomicAdd(&threads, 1u)] = (uint8_t)tid;
     // the sums at one base
     const float block_shift = top == -INFINITY ? 0.0f : -top * BS_LOG2E;
     if (mine != -INFINITY) sum *= bs_ex2(block_shift - shift);      // what had no finite number has a sum of 0, or of NaN
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    const uint32_t values = (end - first + BS_THREADS * W - 1) / (BS_THREADS * W) * W;       // of a thread at the most
+    for (uint32_t x = warp; x < threads; x += 2 * BS_WARPS) {
+        const uint32_t other[2] = {listed[x], x + BS_WARPS < threads ? listed[x + BS_WARPS] : BS_THREADS};
+        for (uint32_t i0 = 0; i0 < values; i0 += 128) {
+            float again[8];
+            uint32_t index[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t i = i0 + (k & 3) * 32 + lane;
+                index[k] = first + ((i / W) * BS_THREADS + other[k >> 2]) * W + i % W;
+                again[k] = i < values && other[k >> 2] < BS_THREADS && index[k] < end ? to_f32(row[index[k]]) : -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (again[k] >= low) {
+                    const uint32_t at = atomicAdd(&count, 1u);
+                    if (at < 2 * BS_THREADS) gathered[at] = bs_key(again[k], index[k]);
+                }
+        }
+    }
     __syncthreads();
     uint32_t kept = count;
     __syncthreads();
@@ -452,29 +498,29 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
     if (tid < keep) lists[(uint64_t)blockIdx.x * keep + tid] = tid < kept ? best[tid] : 0;
     if (!tickets) return;
     // the block that comes last joins the group's runs
-    __threadfence();
     __syncthreads();
     const uint32_t group = row_number / b.beams;
-    if (tid == 0) count = atomicAdd(tickets + group, 1u) + 1 == shape.lists;
+    if (tid == 0) {
+        __threadfence();             // with the barriers before and behind it, for all of the block
+        count = atomicAdd(tickets + group, 1u) + 1 == shape.lists;
+        if (count) tickets[group] = 0;
+        __threadfence();
+    }
     __syncthreads();
     if (!count) return;
-    __threadfence();
-    if (tid == 0) tickets[group] = 0;
-    __syncthreads();
     beam_merge(b, group, row_runs, shape, room, staged, runs, lists, reinterpret_cast<BeamCandidate*>(gathered));
 }
 
 // ---- launch --------------------------------------------------------------------------------------------------------------------
 struct BeamPlan {
-    uint32_t per, run, runs;      // values of a thread at a time; values of a run; runs of a row
+    uint32_t run, runs;      // values of a run; runs of a row
 };
-// Runs so long that about four blocks per SM cover all rows (what comes behind the reading is paid per run), but no longer than a few pieces of 32 values a
-// thread; few rows: pieces of 16 or 8 values.  Multiples of 16 values, so that 16-byte loads stay whole.
+// Runs so long that about two blocks per SM cover all rows: what comes behind the reading is paid per run.  Multiples of 16 values, so that a piece is whole
+// 16-byte units behind its first value.
 static BeamPlan beam_plan(uint64_t rows, uint32_t vocab) {
-    BeamPlan p{32, 0, 0};
     const uint64_t wanted = std::min<uint64_t>(BS_RUNS, std::max<uint64_t>(1, BS_BLOCKS / std::max<uint64_t>(1, rows)));
-    while (p.per > 8 && ceil_div(vocab, p.per * BS_THREADS) < wanted) p.per /= 2;
-    p.runs = (uint32_t)std::min<uint64_t>(wanted, ceil_div(vocab, p.per * BS_THREADS));
+    BeamPlan p;
+    p.runs = (uint32_t)std::min<uint64_t>(wanted, ceil_div(vocab, BS_LEAST_RUN));
     p.run = ceil_div(ceil_div(vocab, p.runs), 16u) * 16;
     p.runs = ceil_div(vocab, p.run);
     return p;
@@ -486,14 +532,12 @@ uint64_t beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t v
 }
 
 template <typename T>
-static void launch_scan(const BeamSelect& b, const BeamPlan& p, BeamRun* runs, uint64_t* lists, const MergeShape& shape, uint32_t room, bool staged,
+static int launch_scan(const BeamSelect& b, const BeamPlan& p, BeamRun* runs, uint64_t* lists, const MergeShape& shape, uint32_t room, bool staged,
                         uint32_t* tickets, cudaStream_t stream) {
-    const dim3 grid(b.groups * b.beams * p.runs);
-    const bool vec = (uintptr_t)b.logits % 16 == 0 && b.logits_ld * sizeof(T) % 16 == 0;
-    auto go = [&](auto kernel) { launch_kernel(kernel, grid, dim3(BS_THREADS), 0, stream, b, p.run, p.runs, runs, lists, shape, room, staged, tickets); };
-    if (p.per == 32) vec ? go(beam_scan_kernel<T, 32, true>) : go(beam_scan_kernel<T, 32, false>);
-    else if (p.per == 16) vec ? go(beam_scan_kernel<T, 16, true>) : go(beam_scan_kernel<T, 16, false>);
-    else vec ? go(beam_scan_kernel<T, 8, true>) : go(beam_scan_kernel<T, 8, false>);
+    if (int rc = allow_shared<beam_scan_kernel<T>>(BeamStage<T>::SPACE, "beam_select attribute")) return rc;
+    launch_kernel(beam_scan_kernel<T>, dim3(b.groups * b.beams * p.runs), dim3(BS_THREADS), BeamStage<T>::SPACE, stream, b, p.run, p.runs, runs, lists, shape, room, staged, tickets,
+                  g_wait_limit_ns.load(std::memory_order_relaxed));
+    return TNSR_B200_OK;
 }
 
 int launch_beam_select(const BeamSelect& b, int dtype, cudaStream_t stream) {
@@ -506,12 +550,13 @@ int launch_beam_select(const BeamSelect& b, int dtype, cudaStream_t stream) {
     const uint32_t room = merge_room(shape, b.keep), bytes = (uint32_t)sizeof(BeamCandidate) * (shape.lists + room), list_bytes = shape.lists * b.keep * 8;
     // joined by a group's last block where that has the shared memory for it, else by a launch of its own
     const bool joined = bytes + list_bytes <= BS_GATHER * 8, staged = joined || list_bytes <= BS_STAGED;
-    if (dtype == TNSR_B200_F32) launch_scan<float>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream);
-    else launch_scan<bf16>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream);
+    int rc = dtype == TNSR_B200_F32 ? launch_scan<float>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream)
+                                    : launch_scan<bf16>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream);
+    if (rc) return rc;
     count_launch();
-    if (int rc = check_launch("beam_select")) return rc;
+    if ((rc = check_launch("beam_select"))) return rc;
     if (joined) return TNSR_B200_OK;
-    if (int rc = allow_shared<beam_merge_kernel>(16 * (BEAM_MAX * BS_RUNS + BEAM_MAX_KEEP * (BEAM_MAX_KEEP + 1)) + BS_STAGED, "beam_select attribute")) return rc;
+    if ((rc = allow_shared<beam_merge_kernel>(16 * (BEAM_MAX * BS_RUNS + BEAM_MAX_KEEP * (BEAM_MAX_KEEP + 1)) + BS_STAGED, "beam_select attribute"))) return rc;
     launch_kernel(beam_merge_kernel, dim3(b.groups), dim3(BS_THREADS), bytes + (staged ? list_bytes : 0), stream, b, p.runs, shape, room, staged, runs, lists);
     count_launch();
     return check_launch("beam_select");

@@ -201,12 +201,15 @@ template <int W, typename T>
 __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
     __shared__ uint32_t s_last;
     const uint32_t c0 = (uint32_t)(unit_at / run.length), c1 = (uint32_t)((unit_at + u.tiles - 1) / run.length), parts = c1 - c0 + 1;
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) s_last = atomicAdd(done + c0, 1u) + 1 == parts;
+    if (threadIdx.x == 0) {
+        __threadfence();             // with the barriers before and behind it, for all of the block
+        s_last = atomicAdd(done + c0, 1u) + 1 == parts;
+        if (s_last) done[c0] = 0;
+        __threadfence();
+    }
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t r = threadIdx.x >> 5; r < u.rows; r += 4) {
         auto part = [&](uint32_t i) { return partial + (((uint64_t)(c0 + i) * 2 + (i == 0)) * 16 + r) * (W + 2); };
@@ -247,7 +250,6 @@ __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u,
             if (c + 1 < p.a.vdim) out[c + 1] = from_f32<T>(v[j].y * inv);
         }
     }
-    if (threadIdx.x == 0) done[c0] = 0;
 }
 
 // bf16 on mma.sync: a tile is 64 keys.  Scores: a warp has 16 keys and all 16 rows; the value product: a warp has a quarter of the columns and all

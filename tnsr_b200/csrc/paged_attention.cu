@@ -5,10 +5,9 @@
 
 #include "mixers.cuh"
 #include "paged.cuh"
+#include "tc_common.cuh"
 
 namespace tb {
-
-constexpr uint32_t PA_NONE = 0xffffffffu;
 
 // The sequence of a row, and the row's place in it.
 __device__ __forceinline__ uint32_t sequence_of(const PagedAttention& a, uint32_t row) {
@@ -110,11 +109,24 @@ struct FewCursor {
     __device__ __forceinline__ uint32_t key0() const { return (tile < u.head_tiles ? tile : u.gap + tile - u.head_tiles) * TK; }
 };
 
+// The four warps that compute; a fifth one feeds them.
+__device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool few_any(bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any) : "r"((uint32_t)x) : "memory");
+    return any != 0;
+}
+
 struct FewRun {
     uint64_t begin, end, length;         // of this block; tiles of a run
 };
 
-// Prefix sums over 128 threads.
+// Prefix sums over the first 128 threads.
 __device__ __forceinline__ uint64_t scan128(uint64_t v, uint64_t* warps, uint64_t& total) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint64_t x = v;
@@ -123,7 +135,7 @@ __device__ __forceinline__ uint64_t scan128(uint64_t v, uint64_t* warps, uint64_
         const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
     }
-    if (lane == 31) warps[warp] = x;
+    if (lane == 31 && warp < 4) warps[warp] = x;
     __syncthreads();
     uint64_t before = 0;
     total = 0;
@@ -140,7 +152,7 @@ template <uint32_t TK>
 __device__ __forceinline__ bool few_plan(const PagedParams& p, bool whole, FewRun& run, FewCursor<TK>& c) {
     __shared__ uint64_t warps[4], s_at;
     __shared__ uint32_t s_sequence;
-    const uint32_t share = (p.a.sequences + 127) / 128, s0 = min(p.a.sequences, threadIdx.x * share), s1 = min(p.a.sequences, s0 + share);
+    const uint32_t share = (p.a.sequences + 127) / 128, s0 = threadIdx.x < 128 ? min(p.a.sequences, threadIdx.x * share) : p.a.sequences, s1 = min(p.a.sequences, s0 + share);
     uint64_t mine = 0;
     for (c.u.s = s0; c.u.s < s1; ++c.u.s) {
         load_sequence<TK>(p, c.u);
@@ -201,14 +213,14 @@ template <int W, typename T>
 __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
     __shared__ uint32_t s_last;
     const uint32_t c0 = (uint32_t)(unit_at / run.length), c1 = (uint32_t)((unit_at + u.tiles - 1) / run.length), parts = c1 - c0 + 1;
-    __syncthreads();
+    few_sync();
     if (threadIdx.x == 0) {
         __threadfence();             // with the barriers before and behind it, for all of the block
         s_last = atomicAdd(done + c0, 1u) + 1 == parts;
         if (s_last) done[c0] = 0;
         __threadfence();
     }
-    __syncthreads();
+    few_sync();
     if (!s_last) return;
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t r = threadIdx.x >> 5; r < u.rows; r += 4) {
@@ -252,92 +264,170 @@ __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u,
     }
 }
 
-// bf16 on mma.sync: a tile is 64 keys.  Scores: a warp has 16 keys and all 16 rows; the value product: a warp has a quarter of the columns and all
-// 64 keys, so that nothing is left to be added up between the warps but the sums of the weights.  Tiles arrive by 16-byte asynchronous
-// copies, STAGES - 1 of them ahead; lane l < 16 of a warp looks up the place of one of its 16 rows a tile before that is asked for.
-// Weights enter the value product as two bf16 pieces (16 bits): the kernel waits for memory, not for the tensor cores.
-// A tile that some rows see only in part may hold infinities or NaN in values that are hidden from others, which a weight of 0 does not
-// keep out: its values are looked through, and if there are any its product is made key by key for each row.
-// STAGES: three of 64 keys keep 64 KB per SM on their way with widths of 128 (two blocks per SM) and 64 (three).
-template <int W, int STAGES>
+// Shared memory: STAGES tiles of keys and values, rows in parts of 128 bytes whose 16-byte pieces lie at (piece ^ row % 8), so that neither eight rows of a
+// piece nor eight pieces of a row meet in a bank.  K and V of a tile are W * 128 bytes each: 64 keys in bf16, 32 in f32.
+template <typename T, int W>
 struct FewShape {
-    static constexpr uint32_t PITCH = W * 2 + 16, TILE = 64 * PITCH, STAGE = 2 * TILE;
-    static constexpr uint32_t P_PITCH = 64 * 2 + 16, P_BYTES = 2 * 16 * P_PITCH;
-    static constexpr uint32_t BYTES = STAGES * STAGE + P_BYTES + 2 * 4 * 16 * 4;
+    static constexpr uint32_t KEYS = 128 / sizeof(T), PART = KEYS * 128, PARTS = W * sizeof(T) / 128, TILE = PART * PARTS;
+    static constexpr uint32_t STAGES = W == 64 ? 4 : 3, RING = STAGES * 2 * TILE;
+    __device__ static __forceinline__ uint32_t at(uint32_t row, uint32_t piece) { return (piece >> 3) * PART + row * 128 + (((piece ^ row) & 7) << 4); }
 };
+// Barriers of the ring, and what is behind them in shared memory.
+template <typename T, int W>
+struct FewRing {
+    uint8_t* tiles;
+    uint64_t *full, *empty;
+    volatile int* abort_flag;
+    __device__ __forceinline__ FewRing(uint8_t* raw) {
+        tiles = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+        full = reinterpret_cast<uint64_t*>(tiles + FewShape<T, W>::RING);
+        empty = full + FewShape<T, W>::STAGES;
+        abort_flag = reinterpret_cast<volatile int*>(empty + FewShape<T, W>::STAGES);
+    }
+};
+constexpr uint32_t FEW_RING_EXTRA = 1024 + 128;      // alignment; barriers and the flag
 
-template <int W, int STAGES, bool UPPER>
-__global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* partial, uint32_t* done) {
-    using S = FewShape<W, STAGES>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint8_t* weights = smem + STAGES * S::STAGE;
-    float* tops = reinterpret_cast<float*>(weights + S::P_BYTES);        // [4][16]
-    float* sums = tops + 64;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+// What the fifth warp does: tile after tile of the run into the ring.  TMA: pools are tensors {width, head, row, page}, a box is the largest power of two of rows
+// that divides a page, and lane i asks for box i; a box that nobody sees, or whose page lies outside the pool, gets coordinates outside: zeros.  Else (pages
+// whose rows are no multiple of 8) 16-byte copies, two or one rows a lane.
+template <typename T, int W, bool TMA>
+__device__ __forceinline__ void few_feed(const PagedParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, uint32_t box, const FewRun& run,
+                                         FewCursor<FewShape<T, W>::KEYS> c, bool whole, const FewRing<T, W>& ring, uint64_t limit) {
+    using S = FewShape<T, W>;
+    const PagedAttention& a = p.a;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t n = 0; whole ? c.at < run.end || c.tile : c.at < run.end; ++n) {
+        const uint32_t stage = n % S::STAGES, key0 = c.key0();
+        const uint32_t* entries = a.table + (uint64_t)c.u.s * a.table_ld;
+        uint8_t* tile = ring.tiles + stage * 2 * S::TILE;
+        if (TMA) {
+            const uint32_t boxes = S::KEYS / box, key = key0 + lane * box;
+            int32_t page = (int32_t)a.pool_pages, row = 0;
+            const bool mine = lane < boxes;
+            // the box's first key that may be seen, or its last
+            if (mine && (int32_t)key <= c.u.last && (!a.window || key < a.sinks || (int64_t)key + box - 1 + a.window > c.u.first)) {
+                const uint32_t i = p.page.div(key), entry = entries[i];
+                row = (int32_t)(key - i * p.page.d);
+                if (entry < a.pool_pages) page = (int32_t)entry;
+                else report(a.d_status, DEV_BAD_PAGE);
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(ring.empty + stage, ((n / S::STAGES) & 1) ^ 1, ring.abort_flag, limit))) return;
+            if (lane == 0) mbar_expect_tx(ring.full + stage, 2 * S::TILE);
+            __syncwarp();
+            if (mine)
+#pragma unroll
+                for (uint32_t part = 0; part < S::PARTS; ++part) {
+                    const uint32_t dst = smem_u32(tile) + part * S::PART + lane * box * 128;
+                    tma_load_4d(dst, map_k, (int32_t)(part * 128 / sizeof(T)), (int32_t)c.u.kvh, row, page, ring.full + stage);
+                    tma_load_4d(dst + S::TILE, map_v, (int32_t)(part * 128 / sizeof(T)), (int32_t)c.u.kvh, row, page, ring.full + stage);
+                }
+        } else {
+            constexpr uint32_t ROWS = S::KEYS / 32, PIECES = W * sizeof(T) / 16, PER = 16 / sizeof(T);
+            const T *k[ROWS], *v[ROWS];
+#pragma unroll
+            for (uint32_t r = 0; r < ROWS; ++r) {
+                const uint32_t key = key0 + r * 32 + lane;
+                k[r] = v[r] = nullptr;
+                if (!unit_sees(p, c.u, key)) continue;
+                uint32_t page, row;
+                if (paged_key(p, entries, key, page, row)) {
+                    k[r] = reinterpret_cast<const T*>(a.k_pool) + a.k_page * page + a.k_row * row + a.k_head * c.u.kvh;
+                    v[r] = reinterpret_cast<const T*>(a.v_pool) + a.v_page * page + a.v_row * row + a.v_head * c.u.kvh;
+                } else {
+                    report(a.d_status, DEV_BAD_PAGE);
+                }
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(ring.empty + stage, ((n / S::STAGES) & 1) ^ 1, ring.abort_flag, limit))) return;
+#pragma unroll
+            for (uint32_t r = 0; r < ROWS; ++r)
+#pragma unroll 8
+                for (uint32_t i = 0; i < PIECES; ++i) {
+                    const uint32_t dst = S::at(r * 32 + lane, i);
+                    const bool k_there = k[r] && i * PER < a.dim, v_there = v[r] && i * PER < a.vdim;
+                    mx_cp16(tile + dst, k_there ? k[r] + i * PER : reinterpret_cast<const T*>(a.k_pool), k_there);
+                    mx_cp16(tile + S::TILE + dst, v_there ? v[r] + i * PER : reinterpret_cast<const T*>(a.v_pool), v_there);
+                }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(ring.full + stage)) : "memory");
+        }
+        c.next(p);
+    }
+    if (!TMA) mx_wait<0>();
+}
+
+// The start of either kernel: barriers, the plan, the fifth warp's work.  False: nothing (more) to do for this thread.
+template <typename T, int W, bool TMA>
+__device__ __forceinline__ bool few_begin(const PagedParams& p, const CUtensorMap* map_k, const CUtensorMap* map_v, uint32_t box, bool whole, const FewRing<T, W>& ring,
+                                          uint64_t limit, FewRun& run, FewCursor<FewShape<T, W>::KEYS>& c) {
+    using S = FewShape<T, W>;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < S::STAGES; ++i) {
+            mbar_init(ring.full + i, TMA ? 1 : 32);
+            mbar_init(ring.empty + i, 4);
+        }
+        *ring.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     pdl_wait();
     pdl_trigger();
-    FewRun run;
-    FewCursor<64> ahead;
-    if (!few_plan<64>(p, partial == nullptr, run, ahead)) return;
-    FewCursor<64> c = ahead;
-    const PagedAttention& a = p.a;
-    // one unit at the end of the run, where runs end with units
-    auto over = [&](const FewCursor<64>& x) { return partial ? x.at >= run.end : x.at >= run.end && x.tile == 0; };
-
-    // row (lane / 2) * 8 + warp * 2 + lane % 2 of the tile ahead, lanes 0 .. 15: its page (or a mark that it is not wanted) and its row there
-    uint32_t page = PA_NONE, row = 0, kvh_ahead = 0;
-    bool wanted = false, more = true;
-    auto look_up = [&]() {
-        wanted = false;
-        more = !over(ahead);
-        if (!more) return;
-        const uint32_t key = ahead.key0() + (lane >> 1) * 8 + warp * 2 + (lane & 1);
-        kvh_ahead = ahead.u.kvh;
-        if (lane < 16 && unit_sees(p, ahead.u, key)) {
-            const uint32_t i = p.page.div(key);
-            row = key - i * p.page.d;
-            page = a.table[(uint64_t)ahead.u.s * a.table_ld + i];
-            wanted = true;
-        }
-        ahead.next(p);
-    };
-    constexpr uint32_t CH = W / 8;               // 16-byte pieces of a row
-    auto load = [&](uint32_t stage) {
-        if (more) {
-            uint64_t k_at = 0, v_at = 0;
-            bool real = wanted && page < a.pool_pages;
-            if (wanted && !real) report(a.d_status, DEV_BAD_PAGE);
-            if (real) {
-                k_at = a.k_page * page + a.k_row * row + a.k_head * kvh_ahead;
-                v_at = a.v_page * page + a.v_row * row + a.v_head * kvh_ahead;
-            }
-            uint8_t* dst = smem + stage * S::STAGE;
-            // the warp copies its own 16 rows, 32 / CH of them at a time
+    if (!few_plan<S::KEYS>(p, whole, run, c)) return false;      // with barriers of the whole block
+    if (threadIdx.x < 128) return true;
+    few_feed<T, W, TMA>(p, map_k, map_v, box, run, c, whole, ring, limit);
+    return false;
+}
+// A wait that gave up: what was computed since is not to be used.  Copies that are still on their way get time to land.
+__device__ __forceinline__ void few_end(const PagedParams& p, volatile int* abort_flag) {
+    if (!*abort_flag) return;
+    const uint64_t start = global_timer_ns();
+    while (global_timer_ns() - start < 200000ull) __nanosleep(1000);
+    if (threadIdx.x == 0) report(p.a.d_status, DEV_TIMEOUT);
+}
+// Values of a tile that some rows see and others do not: rows that nobody sees become zeros (their page may be somebody else's by now); whether one of the others
+// holds infinities or NaN while the rows do not all see the same.
+template <typename T, int W>
+__device__ __forceinline__ bool few_odd_values(const PagedParams& p, const FewUnit& u, uint32_t key0, uint8_t* values) {
+    using S = FewShape<T, W>;
+    bool odd = false;
+    for (uint32_t i = threadIdx.x; i < S::TILE / 16; i += 128) {
+        const uint32_t row = i / (W * sizeof(T) / 16), piece = i % (W * sizeof(T) / 16);
+        uint4* x = reinterpret_cast<uint4*>(values + S::at(row, piece));
+        if (!unit_sees(p, u, key0 + row)) {
+            *x = make_uint4(0u, 0u, 0u, 0u);
+        } else if (u.first != u.last) {
+            const uint4 v = *x;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (uint32_t i = 0; i < 16 * CH / 32; ++i) {
-                const uint32_t piece = i * 32 + lane, owner = piece / CH, ch = piece % CH;
-                const uint64_t k_row = __shfl_sync(0xffffffffu, k_at, owner), v_row = __shfl_sync(0xffffffffu, v_at, owner);
-                const bool there = __shfl_sync(0xffffffffu, (int)real, owner);
-                const uint32_t r = (owner >> 1) * 8 + warp * 2 + (owner & 1);
-                mx_cp16(dst + r * S::PITCH + ch * 16, reinterpret_cast<const bf16*>(a.k_pool) + k_row + (there && ch * 8 < a.dim ? ch * 8 : 0),
-                        there && ch * 8 < a.dim);
-                mx_cp16(dst + S::TILE + r * S::PITCH + ch * 16, reinterpret_cast<const bf16*>(a.v_pool) + v_row + (there && ch * 8 < a.vdim ? ch * 8 : 0),
-                        there && ch * 8 < a.vdim);
-            }
+            for (int e = 0; e < 4; ++e)
+                odd |= sizeof(T) == 4 ? (w[e] & 0x7f800000u) == 0x7f800000u : ((((w[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0);
         }
-        mx_commit();
-    };
-    look_up();
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        load(i);
-        look_up();
     }
+    return odd;
+}
+
+// bf16 on mma.sync: a tile is 64 keys.  Scores: a warp has 16 keys and all 16 rows; the value product: a warp has a quarter of the columns and all
+// 64 keys, so that nothing is left to be added up between the warps but the sums of the weights.  Weights enter the value product as two bf16 pieces
+// (16 bits): the kernel waits for memory, not for the tensor cores.  Values that are hidden from some rows of a tile may be infinities or NaN, which a weight
+// of 0 does not keep out: such a tile's product is made key by key for each row.
+// The ring keeps 64 to 192 KB per SM on their way: four tiles at widths of 64 (three blocks per SM), three at 128 (two) and 256 (one).
+constexpr uint32_t FEW_P_PITCH = 64 * 2 + 16, FEW_P_BYTES = 2 * 16 * FEW_P_PITCH;
+
+template <int W, bool UPPER, bool TMA>
+__global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                        const __grid_constant__ PagedParams p, uint32_t box, float* partial, uint32_t* done, uint64_t limit) {
+    using S = FewShape<bf16, W>;
+    extern __shared__ uint8_t smem[];
+    __shared__ __align__(16) uint8_t weights[FEW_P_BYTES];
+    __shared__ float tops[64], sums[64];                                 // [4][16]
+    const FewRing<bf16, W> ring(smem);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+    FewRun run;
+    FewCursor<64> c;
+    if (!few_begin<bf16, W, TMA>(p, &map_k, &map_v, box, partial == nullptr, ring, limit, run, c)) return;
+    const PagedAttention& a = p.a;
 
     uint32_t qa[W / 16][4];
     float o[W / 32][4], m0, m1, l0, l1;
     int32_t at0, at1;                    // positions of rows g8 and g8 + 8
-    uint64_t unit_at = c.at - c.tile;
+    uint64_t unit_at;
     auto begin_unit = [&]() {
         unit_at = c.at - c.tile;
         const int32_t base = (int32_t)c.u.seq.length - (int32_t)c.u.seq.count;
@@ -377,7 +467,7 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
             sums[warp * 16 + g8] = l0;
             if (UPPER) sums[warp * 16 + g8 + 8] = l1;
         }
-        __syncthreads();
+        few_sync();
         const bool all = unit_at >= run.begin && c.tile + 1 == c.u.tiles;      // c stands at the unit's last tile in this run
 #pragma unroll
         for (int half = 0; half < (UPPER ? 2 : 1); ++half) {
@@ -407,25 +497,24 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
         return all;
     };
     begin_unit();
-    uint32_t stage = 0;
-    while (true) {
-        mx_wait<STAGES - 2>();
-        __syncthreads();
-        load((stage + STAGES - 1) % STAGES);         // where the tile before this one was
-        look_up();
-        const uint8_t* tile = smem + stage * S::STAGE;
-        const uint32_t sk = mx_smem(tile), sv = sk + S::TILE, key0 = c.key0();
+    for (uint32_t n = 0;; ++n) {
+        const uint32_t stage = n % S::STAGES, key0 = c.key0();
+        uint8_t* tile = ring.tiles + stage * 2 * S::TILE;
+        mbar_wait(ring.full + stage, (n / S::STAGES) & 1, ring.abort_flag, limit);      // given up: the run goes on without waiting
+        const uint32_t sk = smem_u32(tile), sv = sk + S::TILE;
         float sc[2][4] = {}, odd[2][4] = {};
+        {
+            const uint32_t key = warp * 16 + (lane & 7) + (lane >> 4) * 8, piece = (lane >> 3) & 1;
 #pragma unroll
-        for (int k = 0; k < W / 16; k += 2) {
-            uint32_t b[4], d[4];
-            const uint32_t at = sk + (warp * 16 + (lane & 7) + (lane >> 4) * 8) * S::PITCH + ((lane >> 3) & 1) * 16 + k * 32;
-            mx_ldsm(at, b);
-            mx_ldsm(at + 32, d);
-            mx_mma(sc[0], qa[k], b[0], b[1]);
-            mx_mma(sc[1], qa[k], b[2], b[3]);
-            mx_mma(odd[0], qa[k + 1], d[0], d[1]);
-            mx_mma(odd[1], qa[k + 1], d[2], d[3]);
+            for (int k = 0; k < W / 16; k += 2) {
+                uint32_t b[4], d[4];
+                mx_ldsm(sk + S::at(key, k * 2 + piece), b);
+                mx_ldsm(sk + S::at(key, k * 2 + 2 + piece), d);
+                mx_mma(sc[0], qa[k], b[0], b[1]);
+                mx_mma(sc[1], qa[k], b[2], b[3]);
+                mx_mma(odd[0], qa[k + 1], d[0], d[1]);
+                mx_mma(odd[1], qa[k + 1], d[2], d[3]);
+            }
         }
         const bool partly = (int64_t)key0 + 63 > c.u.first || (a.window && (int64_t)key0 + a.window <= c.u.last);
         float top0 = -INFINITY, top1 = -INFINITY;
@@ -448,13 +537,13 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
             tops[warp * 16 + g8] = top0;
             if (UPPER) tops[warp * 16 + g8 + 8] = top1;
         }
-        __syncthreads();
+        few_sync();
         auto weigh = [&](int half, float& m, float& l) {
             const float* t = tops + half * 8 + g8;
             const float top = fmaxf(fmaxf(m, fmaxf(t[0], t[16])), fmaxf(t[32], t[48])), ms = top == -INFINITY ? 0.0f : top, f = mx_ex2(m - ms);
             m = top;
             float sum = 0.0f;
-            uint8_t* dst = weights + (half * 8 + g8) * S::P_PITCH + (warp * 16 + t4 * 2) * 2;
+            uint8_t* dst = weights + (half * 8 + g8) * FEW_P_PITCH + (warp * 16 + t4 * 2) * 2;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const float x = mx_ex2(sc[n][2 * half] - ms), y = mx_ex2(sc[n][2 * half + 1] - ms);
@@ -462,7 +551,7 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
                 uint32_t hi, lo;
                 split_bf16x2(x, y, hi, lo);
                 *reinterpret_cast<uint32_t*>(dst + n * 16) = hi;
-                *reinterpret_cast<uint32_t*>(dst + 16 * S::P_PITCH + n * 16) = lo;
+                *reinterpret_cast<uint32_t*>(dst + 16 * FEW_P_PITCH + n * 16) = lo;
             }
             l = l * f + sum;
 #pragma unroll
@@ -473,26 +562,16 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
         };
         weigh(0, m0, l0);
         if (UPPER) weigh(1, m1, l1);
-        // values that some rows see and others do not
-        bool odd_values = false;
-        if (partly && c.u.first != c.u.last) {
-            for (uint32_t i = threadIdx.x; i < 64 * CH; i += 128) {
-                const uint4 v = *reinterpret_cast<const uint4*>(tile + S::TILE + (i / CH) * S::PITCH + (i % CH) * 16);
-                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd_values |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
-            }
-        }
-        if (__syncthreads_or(odd_values)) {
+        if (few_any(partly && few_odd_values<bf16, W>(p, c.u, key0, tile + S::TILE))) {
             for (uint32_t j = 0; j < 64; ++j) {
 #pragma unroll
                 for (int half = 0; half < (UPPER ? 2 : 1); ++half) {
                     if (!row_sees(p, half ? at1 : at0, key0 + j)) continue;
-                    const uint8_t* w = weights + (half * 8 + g8) * S::P_PITCH + j * 2;
-                    const float x = __bfloat162float(*reinterpret_cast<const bf16*>(w)) + __bfloat162float(*reinterpret_cast<const bf16*>(w + 16 * S::P_PITCH));
+                    const uint8_t* w = weights + (half * 8 + g8) * FEW_P_PITCH + j * 2;
+                    const float x = __bfloat162float(*reinterpret_cast<const bf16*>(w)) + __bfloat162float(*reinterpret_cast<const bf16*>(w + 16 * FEW_P_PITCH));
 #pragma unroll
                     for (int n = 0; n < W / 32; ++n) {
-                        const float2 v = bf16x2_to_f32(*reinterpret_cast<const uint32_t*>(tile + S::TILE + j * S::PITCH + (warp * (W / 4) + n * 8 + t4 * 2) * 2));
+                        const float2 v = bf16x2_to_f32(*reinterpret_cast<const uint32_t*>(tile + S::TILE + S::at(j, (warp * (W / 4) + n * 8) / 8) + t4 * 4));
                         o[n][2 * half] = fmaf(x, v.x, o[n][2 * half]);
                         o[n][2 * half + 1] = fmaf(x, v.y, o[n][2 * half + 1]);
                     }
@@ -502,14 +581,14 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 uint32_t hi[4], lo[4];
-                const uint32_t wa = mx_smem(weights) + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::P_PITCH + k * 32 + (lane >> 4) * 16;
+                const uint32_t wa = mx_smem(weights) + ((lane & 7) + ((lane >> 3) & 1) * 8) * FEW_P_PITCH + k * 32 + (lane >> 4) * 16;
                 mx_ldsm(wa, hi);
-                mx_ldsm(wa + 16 * S::P_PITCH, lo);
+                mx_ldsm(wa + 16 * FEW_P_PITCH, lo);
                 if (!UPPER) hi[1] = hi[3] = lo[1] = lo[3] = 0;
 #pragma unroll
                 for (int n = 0; n < W / 64; ++n) {
                     uint32_t b[4];
-                    mx_ldsm_t(sv + (k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * S::PITCH + (warp * (W / 4) + n * 16 + (lane >> 4) * 8) * 2, b);
+                    mx_ldsm_t(sv + S::at(k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, (warp * (W / 4) + n * 16) / 8 + (lane >> 4)), b);
                     mx_mma(o[2 * n], hi, b[0], b[1]);
                     mx_mma(o[2 * n + 1], hi, b[2], b[3]);
                     mx_mma(o[2 * n], lo, b[0], b[1]);
@@ -517,7 +596,10 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
                 }
             }
         }
-        stage = (stage + 1) % STAGES;
+        // the tile has been read (and, where rows became zeros, written: the copies that follow are another proxy's)
+        if (partly) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ring.empty + stage);
         const bool unit_over = c.tile + 1 == c.u.tiles, run_over = partial ? c.at + 1 >= run.end : unit_over && c.at + 1 >= run.end;
         if (unit_over || run_over) {
             if (!end_unit()) few_join<W, bf16>(p, c.u, unit_at, run, partial, done);
@@ -526,92 +608,33 @@ __global__ void __launch_bounds__(128) paged_few_kernel(PagedParams p, float* pa
         c.next(p);
         if (unit_over) begin_unit();
     }
-    mx_wait<0>();
+    few_end(p, ring.abort_flag);
 }
 
 // f32 on CUDA cores: a tile is 32 keys.  Scores: a thread has a key and the rows warp, warp + 4, ...; the value product: a thread has a column (two
 // at widths of 256; half the keys at 64) and all rows.  RQ: rows of a warp.
-template <int W, int STAGES>
-struct FewShape32 {
-    static constexpr uint32_t PITCH = W * 4 + 16, TILE = 32 * PITCH, STAGE = 2 * TILE;
-    static constexpr uint32_t Q = STAGES * STAGE, P = Q + 16 * W * 4, BYTES = P + 32 * 16 * 4 + (W == 64 ? 64 * 16 * 4 : 0) + 4 * 64;
-};
-
-template <int W, int STAGES, int RQ>
-__global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float* partial, uint32_t* done) {
-    using S = FewShape32<W, STAGES>;
-    extern __shared__ __align__(16) uint8_t smem[];
-    float* sq = reinterpret_cast<float*>(smem + S::Q);
-    float* weights = reinterpret_cast<float*>(smem + S::P);              // [32 keys][16 rows]
-    float* half_sums = weights + 32 * 16;                                // W == 64: [16][64]
-    float* factors = half_sums + (W == 64 ? 64 * 16 : 0);                // [16] each: factors, sums, maxima, positions
-    float *sums = factors + 16, *tops = sums + 16;
-    int32_t* places = reinterpret_cast<int32_t*>(tops + 16);
+template <int W, int RQ, bool TMA>
+__global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few_f32_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                            const __grid_constant__ PagedParams p, uint32_t box, float* partial, uint32_t* done, uint64_t limit) {
+    using S = FewShape<float, W>;
+    extern __shared__ uint8_t smem[];
+    __shared__ __align__(16) float sq[RQ * 4 * W], weights[32 * 16], half_sums[W == 64 ? 64 * 16 : 1];      // weights: [32 keys][16 rows]; half_sums: [16][64]
+    __shared__ float factors[16], sums[16], tops[16];
+    __shared__ int32_t places[16];
+    const FewRing<float, W> ring(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_wait();
-    pdl_trigger();
     FewRun run;
-    FewCursor<32> ahead;
-    if (!few_plan<32>(p, partial == nullptr, run, ahead)) return;
-    FewCursor<32> c = ahead;
+    FewCursor<32> c;
+    if (!few_begin<float, W, TMA>(p, &map_k, &map_v, box, partial == nullptr, ring, limit, run, c)) return;
     const PagedAttention& a = p.a;
-    auto over = [&](const FewCursor<32>& x) { return partial ? x.at >= run.end : x.at >= run.end && x.tile == 0; };
-
-    // row warp * 8 + lane of the tile ahead, lanes 0 .. 7
-    uint32_t page = PA_NONE, row = 0, kvh_ahead = 0;
-    bool wanted = false, more = true;
-    auto look_up = [&]() {
-        wanted = false;
-        more = !over(ahead);
-        if (!more) return;
-        const uint32_t key = ahead.key0() + warp * 8 + lane;
-        kvh_ahead = ahead.u.kvh;
-        if (lane < 8 && unit_sees(p, ahead.u, key)) {
-            const uint32_t i = p.page.div(key);
-            row = key - i * p.page.d;
-            page = a.table[(uint64_t)ahead.u.s * a.table_ld + i];
-            wanted = true;
-        }
-        ahead.next(p);
-    };
-    constexpr uint32_t CH = W / 4;
-    auto load = [&](uint32_t stage) {
-        if (more) {
-            uint64_t k_at = 0, v_at = 0;
-            const bool real = wanted && page < a.pool_pages;
-            if (wanted && !real) report(a.d_status, DEV_BAD_PAGE);
-            if (real) {
-                k_at = a.k_page * page + a.k_row * row + a.k_head * kvh_ahead;
-                v_at = a.v_page * page + a.v_row * row + a.v_head * kvh_ahead;
-            }
-            uint8_t* dst = smem + stage * S::STAGE + warp * 8 * S::PITCH;
-#pragma unroll
-            for (uint32_t i = 0; i < 8 * CH / 32; ++i) {
-                const uint32_t piece = i * 32 + lane, owner = piece / CH, ch = piece % CH;
-                const uint64_t k_row = __shfl_sync(0xffffffffu, k_at, owner), v_row = __shfl_sync(0xffffffffu, v_at, owner);
-                const bool there = __shfl_sync(0xffffffffu, (int)real, owner);
-                mx_cp16(dst + owner * S::PITCH + ch * 16, reinterpret_cast<const float*>(a.k_pool) + k_row + (there && ch * 4 < a.dim ? ch * 4 : 0),
-                        there && ch * 4 < a.dim);
-                mx_cp16(dst + S::TILE + owner * S::PITCH + ch * 16, reinterpret_cast<const float*>(a.v_pool) + v_row + (there && ch * 4 < a.vdim ? ch * 4 : 0),
-                        there && ch * 4 < a.vdim);
-            }
-        }
-        mx_commit();
-    };
-    look_up();
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        load(i);
-        look_up();
-    }
 
     constexpr int COLUMNS = W == 256 ? 2 : 1, KEYS = W == 64 ? 16 : 32;   // of a thread in the value product
     const uint32_t col = tid % W, key_first = W == 64 ? (tid / 64) * 16 : 0;
     float o[COLUMNS][RQ * 4], m[RQ], l[RQ];
-    uint64_t unit_at = c.at - c.tile;
+    uint64_t unit_at;
     auto begin_unit = [&]() {
         unit_at = c.at - c.tile;
-        __syncthreads();                     // the last unit's rows are done with
+        few_sync();                     // the last unit's rows are done with
         const int32_t base = (int32_t)c.u.seq.length - (int32_t)c.u.seq.count;
         for (uint32_t i = tid; i < RQ * 4 * W; i += 128) {
             const uint32_t r = i / W, x = i % W, R = c.u.row0 + min(r, c.u.rows - 1), token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
@@ -643,7 +666,7 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
         if (W == 64 && tid >= 64)
 #pragma unroll
             for (int r = 0; r < RQ * 4; ++r) half_sums[r * 64 + col] = o[0][r];
-        __syncthreads();
+        few_sync();
         const bool all = unit_at >= run.begin && c.tile + 1 == c.u.tiles;
         if (W != 64 || tid < 64) {
 #pragma unroll
@@ -669,19 +692,15 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
         return all;
     };
     begin_unit();
-    uint32_t stage = 0;
-    while (true) {
-        mx_wait<STAGES - 2>();
-        __syncthreads();
-        load((stage + STAGES - 1) % STAGES);
-        look_up();
-        const uint8_t* tile = smem + stage * S::STAGE;
-        const uint32_t key0 = c.key0();
+    for (uint32_t n = 0;; ++n) {
+        const uint32_t stage = n % S::STAGES, key0 = c.key0();
+        uint8_t* tile = ring.tiles + stage * 2 * S::TILE;
+        mbar_wait(ring.full + stage, (n / S::STAGES) & 1, ring.abort_flag, limit);      // given up: the run goes on without waiting
+        few_sync();                          // the rows of a new unit are there, the weights of the last tile have been read
         float dot[RQ] = {};
-        const float4* k = reinterpret_cast<const float4*>(tile + lane * S::PITCH);
 #pragma unroll 8
         for (int x = 0; x < W / 4; ++x) {
-            const float4 kv = k[x];
+            const float4 kv = *reinterpret_cast<const float4*>(tile + S::at(lane, x));
 #pragma unroll
             for (int i = 0; i < RQ; ++i) {
                 const float4 q = reinterpret_cast<const float4*>(sq + (warp + 4 * i) * W)[x];
@@ -700,10 +719,8 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
             weights[lane * 16 + warp + 4 * i] = w;
             if (lane == 0) factors[warp + 4 * i] = f;
         }
-        bool odd_values = false;
-        if (c.u.first != c.u.last && ((int64_t)key0 + 31 > c.u.first || (a.window && (int64_t)key0 + a.window <= c.u.last)))
-            for (uint32_t i = tid; i < 32 * W; i += 128) odd_values |= !isfinite(reinterpret_cast<const float*>(tile + S::TILE + (i / W) * S::PITCH)[i % W]);
-        const bool careful = __syncthreads_or(odd_values);
+        const bool partly = (int64_t)key0 + 31 > c.u.first || (a.window && (int64_t)key0 + a.window <= c.u.last);
+        const bool careful = few_any(partly && few_odd_values<float, W>(p, c.u, key0, tile + S::TILE));
 #pragma unroll
         for (int r = 0; r < RQ * 4; ++r)
 #pragma unroll
@@ -712,7 +729,7 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
         for (int j = 0; j < KEYS; ++j) {
             float v[COLUMNS];
 #pragma unroll
-            for (int n = 0; n < COLUMNS; ++n) v[n] = reinterpret_cast<const float*>(tile + S::TILE + (key_first + j) * S::PITCH)[col + n * 128];
+            for (int n = 0; n < COLUMNS; ++n) v[n] = *reinterpret_cast<const float*>(tile + S::TILE + S::at(key_first + j, (col + n * 128) / 4) + (col % 4) * 4);
             const float4* w = reinterpret_cast<const float4*>(weights + (key_first + j) * 16);
 #pragma unroll
             for (int q = 0; q < RQ; ++q) {
@@ -725,7 +742,10 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
                         for (int n = 0; n < COLUMNS; ++n) o[n][4 * q + e] = fmaf(f[e], v[n], o[n][4 * q + e]);
             }
         }
-        stage = (stage + 1) % STAGES;
+        // the tile has been read (and, where rows became zeros, written: the copies that follow are another proxy's)
+        if (partly) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ring.empty + stage);
         const bool unit_over = c.tile + 1 == c.u.tiles, run_over = partial ? c.at + 1 >= run.end : unit_over && c.at + 1 >= run.end;
         if (unit_over || run_over) {
             if (!end_unit()) few_join<W, float>(p, c.u, unit_at, run, partial, done);
@@ -734,12 +754,11 @@ __global__ void __launch_bounds__(128) paged_few_f32_kernel(PagedParams p, float
         c.next(p);
         if (unit_over) begin_unit();
     }
-    mx_wait<0>();
+    few_end(p, ring.abort_flag);
 }
 
 // ---- launch ------------------------------------------------------------------------------------------------------------------------
 namespace {
-constexpr int FEW_STAGES = 3;
 constexpr uint32_t FEW_ROWS = 64;        // rows (tokens x heads of a group) of a sequence up to which the keys are divided
 
 uint32_t few_width(uint32_t dim, uint32_t vdim) {
@@ -749,8 +768,24 @@ uint32_t few_width(uint32_t dim, uint32_t vdim) {
 // As many blocks as run at once: shared memory lets three (widths of 64), two or one of them on an SM.
 uint32_t few_blocks(uint32_t width) { return 148 * (width == 64 ? 3 : width == 128 ? 2 : 1); }
 
-template <auto KERNEL>
-int launch_few(const PagedParams& p, uint32_t bytes, uint32_t grid, cudaStream_t stream) {
+struct FewLaunch {
+    CUtensorMap k, v;
+    uint32_t box, grid;      // box 0: no tensor maps
+};
+
+// Pools as tensors {width, head, row, page}; boxes of 128 bytes x `box` rows, pieces of 16 bytes exchanged as FewShape::at says.
+bool few_map(CUtensorMap* map, const void* base, int dtype, uint32_t width, const PagedAttention& a, uint64_t head, uint64_t row, uint64_t page, uint32_t box) {
+    const uint64_t size = dtype == TNSR_B200_F32 ? 4 : 2;
+    const cuuint64_t dims[4] = {width, a.kv_heads, a.page_rows, a.pool_pages}, strides[3] = {head * size, row * size, page * size};
+    const cuuint32_t boxes[4] = {(cuuint32_t)(128 / size), 1, box, 1}, ones[4] = {1, 1, 1, 1};
+    return encode_fn()(map, dtype == TNSR_B200_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
+                       ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int W, auto KERNEL>
+int launch_few(const PagedParams& p, const FewLaunch& f, cudaStream_t stream) {
+    constexpr uint32_t bytes = FewShape<T, W>::RING + FEW_RING_EXTRA;
     if (const int rc = allow_shared<KERNEL>(bytes, "paged_attention attribute")) return rc;
     float* partial = nullptr;
     uint32_t* done = nullptr;
@@ -758,20 +793,22 @@ int launch_few(const PagedParams& p, uint32_t bytes, uint32_t grid, cudaStream_t
         done = reinterpret_cast<uint32_t*>(p.a.workspace);
         partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + FEW_COUNTERS);
     }
-    launch_kernel(KERNEL, dim3(grid), dim3(128), bytes, stream, p, partial, done);
+    launch_kernel(KERNEL, dim3(f.grid), dim3(160), bytes, stream, f.k, f.v, p, f.box, partial, done, g_wait_limit_ns.load(std::memory_order_relaxed));
     return TNSR_B200_OK;
 }
-template <int W>
-int launch_few_width(const PagedParams& p, int dtype, uint32_t rows, uint32_t grid, cudaStream_t stream) {
-    if (dtype == TNSR_B200_BF16) {
-        constexpr uint32_t bytes = FewShape<W, FEW_STAGES>::BYTES;
-        return rows > 8 ? launch_few<paged_few_kernel<W, FEW_STAGES, true>>(p, bytes, grid, stream)
-                        : launch_few<paged_few_kernel<W, FEW_STAGES, false>>(p, bytes, grid, stream);
-    }
-    constexpr uint32_t bytes = FewShape32<W, FEW_STAGES>::BYTES;
-    return rows > 8   ? launch_few<paged_few_f32_kernel<W, FEW_STAGES, 4>>(p, bytes, grid, stream)
-           : rows > 4 ? launch_few<paged_few_f32_kernel<W, FEW_STAGES, 2>>(p, bytes, grid, stream)
-                      : launch_few<paged_few_f32_kernel<W, FEW_STAGES, 1>>(p, bytes, grid, stream);
+template <int W, bool TMA>
+int launch_few_width(const PagedParams& p, int dtype, uint32_t rows, const FewLaunch& f, cudaStream_t stream) {
+    if (dtype == TNSR_B200_BF16)
+        return rows > 8 ? launch_few<bf16, W, paged_few_kernel<W, true, TMA>>(p, f, stream) : launch_few<bf16, W, paged_few_kernel<W, false, TMA>>(p, f, stream);
+    return rows > 8   ? launch_few<float, W, paged_few_f32_kernel<W, 4, TMA>>(p, f, stream)
+           : rows > 4 ? launch_few<float, W, paged_few_f32_kernel<W, 2, TMA>>(p, f, stream)
+                      : launch_few<float, W, paged_few_f32_kernel<W, 1, TMA>>(p, f, stream);
+}
+template <bool TMA>
+int launch_few_any(const PagedParams& p, int dtype, uint32_t width, uint32_t rows, const FewLaunch& f, cudaStream_t stream) {
+    return width == 64    ? launch_few_width<64, TMA>(p, dtype, rows, f, stream)
+           : width == 128 ? launch_few_width<128, TMA>(p, dtype, rows, f, stream)
+                          : launch_few_width<256, TMA>(p, dtype, rows, f, stream);
 }
 }  // namespace
 
@@ -802,13 +839,25 @@ int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stre
     } else if (rows > FEW_ROWS && paged_prompt_eligible(a, dtype)) {
         rc = launch_paged_prompt(p, stream);
     } else {
-        const uint32_t w = few_width(a.dim, a.vdim), most = (uint32_t)std::min<uint64_t>(16, rows);
+        const uint32_t w = few_width(a.dim, a.vdim), most = (uint32_t)std::min<uint64_t>(16, rows), keys = dtype == TNSR_B200_F32 ? 32u : 64u;
         // no more blocks than there can be tiles
-        const uint64_t tiles = (uint64_t)a.sequences * a.kv_heads * ceil_div64(rows, 16) * (ceil_div(p.capacity, dtype == TNSR_B200_F32 ? 32u : 64u) + 1);
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, few_blocks(w));
-        rc = w == 64    ? launch_few_width<64>(p, dtype, most, grid, stream)
-             : w == 128 ? launch_few_width<128>(p, dtype, most, grid, stream)
-                        : launch_few_width<256>(p, dtype, most, grid, stream);
+        const uint64_t tiles = (uint64_t)a.sequences * a.kv_heads * ceil_div64(rows, 16) * (ceil_div(p.capacity, keys) + 1);
+        FewLaunch f = {};
+        f.grid = (uint32_t)std::min<uint64_t>(tiles, few_blocks(w));
+        f.box = std::min(keys, a.page_rows & (0u - a.page_rows));
+        const uint64_t largest = std::max({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head}), smallest = std::min({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head});
+        // strides of a tensor map are less than 2^40 bytes, its coordinates 31 bits
+        const bool tma = f.box >= 8 && smallest > 0 && largest < (1ull << 37) && a.pool_pages < 0x7fffffffu && encode_fn() != nullptr;
+        if (tma) {
+            if (!few_map(&f.k, a.k_pool, dtype, a.dim, a, a.k_head, a.k_row, a.k_page, f.box) ||
+                !few_map(&f.v, a.v_pool, dtype, a.vdim, a, a.v_head, a.v_row, a.v_page, f.box)) {
+                set_thread_error("paged_attention: tensor map encoding failed");
+                return TNSR_B200_ERR_CUDA;
+            }
+            rc = launch_few_any<true>(p, dtype, w, most, f, stream);
+        } else {
+            rc = launch_few_any<false>(p, dtype, w, most, f, stream);
+        }
     }
     if (rc) return rc;
     count_launch();

@@ -101,10 +101,6 @@ __device__ __forceinline__ void pp_load_3d(uint32_t dst, const CUtensorMap* map,
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
-__device__ __forceinline__ void pp_load_4d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
 
 // Two values at once.
 __device__ __forceinline__ uint64_t pp_pair(float x, float y) {
@@ -283,7 +279,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (lane < boxes)
 #pragma unroll
                     for (uint32_t h = 0; h < HALVES; ++h)
-                        pp_load_4d(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_k, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
+                        tma_load_4d(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_k, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
                                    k_full + stage);
                 if (j == 0) {
                     for (int t = 0; t < 2 && ok; ++t) {
@@ -308,7 +304,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (lane < boxes)
 #pragma unroll
                     for (uint32_t h = 0; h < HALVES; ++h)
-                        pp_load_4d(smem_u32(v_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_v, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
+                        tma_load_4d(smem_u32(v_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_v, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
                                    v_full + stage);
             }
         }

@@ -2,6 +2,7 @@
 // position p sees keys j <= p with j > p - window, and the first `sinks` ones beside the window; window 0: all of them.  The rows of a
 // sequence are the last of its keys; a row before its first key sees nothing and gives zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "mixers.cuh"
 #include "paged.cuh"
@@ -122,6 +123,11 @@ __device__ __forceinline__ bool few_any(bool x) {
     return any != 0;
 }
 
+// x / y, by 32 bits where they do: 64 take some hundred instructions, and every block divides when it plans.
+__device__ __forceinline__ uint64_t few_div(uint64_t x, uint64_t y) {
+    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
+}
+
 struct FewRun {
     uint64_t begin, end, length;         // of this block; tiles of a run
 };
@@ -151,36 +157,45 @@ __device__ __forceinline__ uint64_t scan128(uint64_t v, uint64_t* warps, uint64_
 template <uint32_t TK>
 __device__ __forceinline__ bool few_plan(const PagedParams& p, bool whole, FewRun& run, FewCursor<TK>& c) {
     __shared__ uint64_t warps[4], s_at;
-    __shared__ uint32_t s_sequence;
+    __shared__ uint32_t s_sequence, s_per_head;
+    __shared__ PagedSequence s_found;
     const uint32_t share = (p.a.sequences + 127) / 128, s0 = threadIdx.x < 128 ? min(p.a.sequences, threadIdx.x * share) : p.a.sequences, s1 = min(p.a.sequences, s0 + share);
     uint64_t mine = 0;
+    uint32_t per_head = 0;
     for (c.u.s = s0; c.u.s < s1; ++c.u.s) {
         load_sequence<TK>(p, c.u);
-        mine += (uint64_t)head_tiles<TK>(p, c.u) * p.a.kv_heads;
+        per_head = head_tiles<TK>(p, c.u);
+        mine += (uint64_t)per_head * p.a.kv_heads;
     }
     uint64_t total;
     uint64_t before = scan128(mine, warps, total);
-    run.length = max((uint64_t)1, (total + gridDim.x - 1) / gridDim.x);
+    run.length = max((uint64_t)1, few_div(total + gridDim.x - 1, gridDim.x));
     run.begin = blockIdx.x * run.length;
     run.end = min(total, run.begin + run.length);
     if (run.begin >= total) return false;
     if (run.begin >= before && run.begin < before + mine) {
-        for (c.u.s = s0; c.u.s < s1; ++c.u.s) {
-            load_sequence<TK>(p, c.u);
-            const uint64_t n = (uint64_t)head_tiles<TK>(p, c.u) * p.a.kv_heads;
-            if (run.begin < before + n) break;
-            before += n;
-        }
+        c.u.s = s0;
+        if (share > 1)
+            for (;; ++c.u.s) {
+                load_sequence<TK>(p, c.u);
+                per_head = head_tiles<TK>(p, c.u);
+                const uint64_t n = (uint64_t)per_head * p.a.kv_heads;
+                if (run.begin < before + n) break;
+                before += n;
+            }
         s_sequence = c.u.s;
+        s_found = c.u.seq;
+        s_per_head = per_head;
         s_at = before;
     }
     __syncthreads();
     c.u.s = s_sequence;
-    load_sequence<TK>(p, c.u);
-    uint64_t rest = run.begin - s_at;
-    const uint32_t per_head = head_tiles<TK>(p, c.u);
-    c.u.kvh = (uint32_t)(rest / per_head);
-    uint32_t r = (uint32_t)(rest % per_head);
+    c.u.seq = s_found;
+    c.u.row_tiles = (c.u.seq.count * p.per.d + 15) / 16;
+    per_head = s_per_head;
+    const uint64_t rest = run.begin - s_at;
+    c.u.kvh = (uint32_t)few_div(rest, per_head);
+    uint32_t r = (uint32_t)(rest - (uint64_t)c.u.kvh * per_head);
     for (c.u.rt = 0;; ++c.u.rt) {
         unit_tiles<TK>(p, c.u);
         if (r < c.u.tiles) break;
@@ -208,11 +223,10 @@ constexpr uint32_t FEW_COUNTERS = 4096;          // bytes before the partial res
 static_assert(FEW_COUNTERS >= FEW_BLOCKS * 4, "a counter per block");
 
 // Partial results of a unit joined by the block that comes last, in the order of the runs.  Layout [block][whether the unit begins in its run][16][W + 2].
-// A warp per row; lanes hold the factors of 32 parts at a time.
 template <int W, typename T>
 __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
     __shared__ uint32_t s_last;
-    const uint32_t c0 = (uint32_t)(unit_at / run.length), c1 = (uint32_t)((unit_at + u.tiles - 1) / run.length), parts = c1 - c0 + 1;
+    const uint32_t c0 = (uint32_t)few_div(unit_at, run.length), c1 = (uint32_t)few_div(unit_at + u.tiles - 1, run.length), parts = c1 - c0 + 1;
     few_sync();
     if (threadIdx.x == 0) {
         __threadfence();             // with the barriers before and behind it, for all of the block
@@ -222,44 +236,82 @@ __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u,
     }
     few_sync();
     if (!s_last) return;
-    const uint32_t lane = threadIdx.x & 31;
-    for (uint32_t r = threadIdx.x >> 5; r < u.rows; r += 4) {
-        auto part = [&](uint32_t i) { return partial + (((uint64_t)(c0 + i) * 2 + (i == 0)) * 16 + r) * (W + 2); };
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < parts; i += 32) top = fmaxf(top, __ldcg(part(i) + W));
+    // a warp has up to four rows, whose loads are on their way together; lanes hold the factors of 32 parts at a time
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr uint32_t ROW = W + 2;
+    auto part = [&](uint32_t i) { return partial + (((uint64_t)(c0 + i) * 2 + (i == 0)) * 16 + warp) * ROW; };        // row `warp` of it
+    float top[4], sum[4] = {};
+    float2 v[4][W / 64];
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float ms = top == -INFINITY ? 0.0f : top;
+    for (int k = 0; k < 4; ++k) {
+        top[k] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < W / 64; ++j) v[k][j] = make_float2(0.0f, 0.0f);
+    }
+    for (uint32_t i = lane; i < parts; i += 32)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (warp + 4 * k < u.rows) top[k] = fmaxf(top[k], __ldcg(part(i) + 4 * k * ROW + W));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], d));
+    for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
+        const uint32_t n = min(32u, parts - i0);
+        float factor[4] = {};
+        if (lane < n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (warp + 4 * k < u.rows) {
+                    const float2 x = __ldcg(reinterpret_cast<const float2*>(part(i0 + lane) + 4 * k * ROW + W));
+                    factor[k] = mx_ex2(x.x - (top[k] == -INFINITY ? 0.0f : top[k]));
+                    sum[k] = fmaf(factor[k], x.y, sum[k]);
+                }
+        // eight loads a lane on their way: of a row eight parts, or of four rows two
+        auto add = [&](uint32_t i, auto rows_at_once, auto parts_at_once) {
+            constexpr int ROWS = decltype(rows_at_once)::value, PARTS = decltype(parts_at_once)::value;
+            float2 x[PARTS][ROWS][W / 64];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                const float* src = part(i0 + min(i + q, n - 1));
+#pragma unroll
+                for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+                    for (int j = 0; j < W / 64; ++j)
+                        x[q][k][j] = warp + 4 * k < u.rows ? __ldcg(reinterpret_cast<const float2*>(src + 4 * k * ROW) + j * 32 + lane) : make_float2(0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                for (int k = 0; k < ROWS; ++k) {
+                    const float f = __shfl_sync(0xffffffffu, factor[k], (i + q) & 31);
+                    if (i + q >= n) continue;
+#pragma unroll
+                    for (int j = 0; j < W / 64; ++j) {
+                        v[k][j].x = fmaf(f, x[q][k][j].x, v[k][j].x);
+                        v[k][j].y = fmaf(f, x[q][k][j].y, v[k][j].y);
+                    }
+                }
+        };
+        if (u.rows <= 4)
+            for (uint32_t i = 0; i < n; i += 8) add(i, std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
+        else
+            for (uint32_t i = 0; i < n; i += 2) add(i, std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t r = warp + 4 * k;
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
+        if (r >= u.rows) continue;
+        const float inv = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
         const uint32_t R = u.row0 + r, token = p.per.div(R), h = u.kvh * p.per.d + R - token * p.per.d;
         T* out = reinterpret_cast<T*>(p.a.out) + (uint64_t)(u.seq.start + token) * p.a.out_ld + (uint64_t)h * p.a.vdim;
-        float2 v[W / 64];
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W / 64; ++j) v[j] = make_float2(0.0f, 0.0f);
-        for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
-            const uint32_t n = min(32u, parts - i0);
-            const float factor = lane < n ? mx_ex2(__ldcg(part(i0 + lane) + W) - ms) : 0.0f;
-            if (lane < n) sum = fmaf(factor, __ldcg(part(i0 + lane) + W + 1), sum);
-#pragma unroll 4
-            for (uint32_t i = 0; i < n; ++i) {
-                const float f = __shfl_sync(0xffffffffu, factor, i);
-                const float2* src = reinterpret_cast<const float2*>(part(i0 + i));
-#pragma unroll
-                for (int j = 0; j < W / 64; ++j) {
-                    const float2 x = __ldcg(src + j * 32 + lane);
-                    v[j].x = fmaf(f, x.x, v[j].x);
-                    v[j].y = fmaf(f, x.y, v[j].y);
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int j = 0; j < W / 64; ++j) {
             const uint32_t c = j * 64 + lane * 2;
-            if (c < p.a.vdim) out[c] = from_f32<T>(v[j].x * inv);
-            if (c + 1 < p.a.vdim) out[c + 1] = from_f32<T>(v[j].y * inv);
+            if (c < p.a.vdim) out[c] = from_f32<T>(v[k][j].x * inv);
+            if (c + 1 < p.a.vdim) out[c + 1] = from_f32<T>(v[k][j].y * inv);
         }
     }
 }
@@ -725,8 +777,7 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
         for (int r = 0; r < RQ * 4; ++r)
 #pragma unroll
             for (int n = 0; n < COLUMNS; ++n) o[n][r] *= factors[r];
-#pragma unroll 4
-        for (int j = 0; j < KEYS; ++j) {
+        auto product = [&](int j, bool all) {
             float v[COLUMNS];
 #pragma unroll
             for (int n = 0; n < COLUMNS; ++n) v[n] = *reinterpret_cast<const float*>(tile + S::TILE + S::at(key_first + j, (col + n * 128) / 4) + (col % 4) * 4);
@@ -737,10 +788,17 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
                 const float f[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!careful || row_sees(p, places[4 * q + e], key0 + key_first + j))
+                    if (all || row_sees(p, places[4 * q + e], key0 + key_first + j))
 #pragma unroll
                         for (int n = 0; n < COLUMNS; ++n) o[n][4 * q + e] = fmaf(f[e], v[n], o[n][4 * q + e]);
             }
+        };
+        if (careful) {
+#pragma unroll 1
+            for (int j = 0; j < KEYS; ++j) product(j, false);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KEYS; ++j) product(j, true);
         }
         // the tile has been read (and, where rows became zeros, written: the copies that follow are another proxy's)
         if (partly) fence_proxy_async_smem();

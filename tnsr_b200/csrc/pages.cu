@@ -12,7 +12,7 @@
 // The bookkeeping is integers: counters by atomics (sums do not depend on their order), choices by ranks (prefix sums in order of sequences and
 // pages), so a call's result is a function of its inputs.  What has an order runs in one block: 16 sequences x 4 beams with 40 entries each take
 // a few us, which is the latency of a chain of dependent reads, and the search for free pages ends at the last one that is needed.
-// What bounds a call that copies is the copying: 16-byte loads, four on their way per thread.
+// What bounds a call that copies is the copying: 16-byte loads, eight on their way per thread.
 //
 // Also here: rows appended to caches in pages, and states reordered to their sequences' parents.
 #include <algorithm>
@@ -73,27 +73,35 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t& total) {
 }
 
 // ---- fork -----------------------------------------------------------------------------------------------------------------
-// A block has `columns` columns of the whole table in shared memory, so that rows can trade places; the last block to have read the
-// lengths writes them.
+// A block has `columns` columns of the whole table in shared memory, so that rows can trade places, and beside them what everybody's length and parent is; the last
+// block that has read the lengths writes them.
 __global__ void __launch_bounds__(256) pages_fork_kernel(PageBook b, const uint32_t* parents, uint32_t columns, uint32_t* ticket) {
-    extern __shared__ uint32_t staged[];
+    extern __shared__ uint32_t staged[];       // [sequences][columns], [sequences] lengths, [sequences] parents
     __shared__ uint32_t s_last;
+    uint32_t *lengths = staged + columns * b.sequences, *from = lengths + b.sequences;
     pdl_wait();
     pdl_trigger();
     const uint32_t column0 = blockIdx.x * columns, here = min(columns, b.table_ld - column0), cells = b.sequences * here;
+    for (uint32_t s = threadIdx.x; s < b.sequences; s += blockDim.x) {
+        lengths[s] = b.lengths[s];
+        uint32_t p = parents[s];
+        if (p >= b.sequences) {
+            if (blockIdx.x == 0) report(b.d_status, DEV_BAD_PARENT);
+            p = s;
+        }
+        from[s] = p;
+    }
+    __syncthreads();
+    auto live = [&](uint32_t s) { return min(pages_of(lengths[s], b.page_rows), b.table_ld); };
     for (uint32_t i = threadIdx.x; i < cells; i += blockDim.x) {
         const uint32_t s = i / here, c = i % here;
-        staged[i] = column0 + c < live_pages(b, s) ? b.table[(size_t)s * b.table_ld + column0 + c] : PG_NONE;
+        staged[i] = column0 + c < live(s) ? b.table[(size_t)s * b.table_ld + column0 + c] : PG_NONE;
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < cells; i += blockDim.x) {
-        const uint32_t s = i / here, c = i % here, p = parents[s];
-        if (p >= b.sequences) {
-            if (c == 0) report(b.d_status, DEV_BAD_PARENT);
-            continue;
-        }
+        const uint32_t s = i / here, c = i % here, p = from[s];
         if (p == s) continue;
-        const bool was = column0 + c < live_pages(b, s), is = column0 + c < live_pages(b, p);
+        const bool was = column0 + c < live(s), is = column0 + c < live(p);
         const uint32_t before = staged[i], page = staged[p * here + c];
         if (is) b.table[(size_t)s * b.table_ld + column0 + c] = page;
         if (was && is && before == page) continue;
@@ -101,28 +109,21 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(PageBook b, const uint3
         if (was && before < b.pool_pages) atomicSub(b.holders + before, 1u);
         if (is && page < b.pool_pages) atomicAdd(b.holders + page, 1u);
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = atomicAdd(ticket, 1u) + 1 == gridDim.x;
-    }
+    if (threadIdx.x == 0) s_last = atomicAdd(ticket, 1u) + 1 == gridDim.x;      // lengths were read before the first barrier
     __syncthreads();
     if (!s_last) return;
-    for (uint32_t s = threadIdx.x; s < b.sequences; s += blockDim.x) {
-        const uint32_t p = parents[s];
-        staged[s] = b.lengths[p < b.sequences ? p : s];
-    }
-    __syncthreads();
-    for (uint32_t s = threadIdx.x; s < b.sequences; s += blockDim.x) b.lengths[s] = staged[s];
+    for (uint32_t s = threadIdx.x; s < b.sequences; s += blockDim.x)
+        if (from[s] != s) b.lengths[s] = lengths[from[s]];
     if (threadIdx.x == 0) *ticket = 0;
 }
 
 int launch_pages_fork(const PageBook& b, const uint32_t* parents, cudaStream_t stream) {
     if (b.sequences == 0) return TNSR_B200_OK;
-    uint32_t columns = 8;
-    while (columns > 1 && (uint64_t)columns * b.sequences > 12288) columns /= 2;
+    // at most 48 KB of shared memory; few sequences: two columns a block, for less to do one thing behind the other
+    uint32_t columns = b.sequences > 256 ? 8 : 2;
+    while (columns > 1 && (uint64_t)(columns + 2) * b.sequences > 12288) columns /= 2;
     const PageScratch ws = page_scratch(b.workspace, b.sequences, b.pool_pages);
-    launch_kernel(pages_fork_kernel, dim3(ceil_div(b.table_ld, columns)), dim3(256), (size_t)columns * b.sequences * 4, stream, b, parents, columns,
+    launch_kernel(pages_fork_kernel, dim3(ceil_div(b.table_ld, columns)), dim3(256), (size_t)(columns + 2) * b.sequences * 4, stream, b, parents, columns,
                   ws.header + 1);
     count_launch();
     return check_launch("pages_fork");
@@ -130,7 +131,7 @@ int launch_pages_fork(const PageBook& b, const uint32_t* parents, cudaStream_t s
 
 // ---- contents of pages ------------------------------------------------------------------------------------------------------
 constexpr uint32_t PG_POOLS = 64;                // pools of a launch: their pointers travel as parameters
-constexpr uint32_t PG_PIECE = 16384;             // bytes that a block copies at a time
+constexpr uint32_t PG_PIECE = 32768;             // bytes that a block copies at a time: eight 16-byte loads a thread
 struct PoolList {
     uint8_t* at[PG_POOLS];
     uint64_t bytes[PG_POOLS];
@@ -139,19 +140,19 @@ struct PoolList {
     bool wide;                       // 16-byte units
 };
 
-__device__ __forceinline__ void copy_piece(uint8_t* to, const uint8_t* from, uint64_t bytes, bool wide) {
+__device__ __forceinline__ void copy_piece(uint8_t* __restrict__ to, const uint8_t* from, uint64_t bytes, bool wide) {
     if (wide) {
         const uint4* src = reinterpret_cast<const uint4*>(from);
         uint4* dst = reinterpret_cast<uint4*>(to);
         const uint32_t n = (uint32_t)(bytes / 16);
-        for (uint32_t i = threadIdx.x; i < n; i += 4 * blockDim.x) {
-            uint4 v[4];
+        uint4 v[8];
+        for (uint32_t i = threadIdx.x; i < n; i += 8 * 256) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + j * blockDim.x < n) v[j] = src[i + j * blockDim.x];
+            for (int j = 0; j < 8; ++j)
+                if (i + j * 256 < n) v[j] = src[i + j * 256];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + j * blockDim.x < n) dst[i + j * blockDim.x] = v[j];
+            for (int j = 0; j < 8; ++j)
+                if (i + j * 256 < n) dst[i + j * 256] = v[j];
         }
     } else {
         for (uint64_t i = threadIdx.x; i < bytes; i += blockDim.x) to[i] = from[i];
@@ -175,12 +176,28 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
             else if (page >= live) b.table[i] = moved[page];
         }
     }
+    // pair by pair in pieces of all pools; the next item's pages are asked for before the copy
     const uint64_t items = (uint64_t)n * pools.pieces_all;
+    const uint32_t pairs_on = gridDim.x / max(pools.pieces_all, 1u), pieces_on = gridDim.x - pairs_on * pools.pieces_all;
+    uint32_t pair = blockIdx.x / max(pools.pieces_all, 1u), at = blockIdx.x - pair * pools.pieces_all, next_src = 0, next_dst = 0;
+    if (blockIdx.x < items) {
+        next_src = from[pair];
+        next_dst = to[pair];
+    }
     for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t pair = (uint32_t)(item / pools.pieces_all);
-        uint32_t piece = (uint32_t)(item % pools.pieces_all), t = 0;
+        const uint32_t src = next_src, dst = next_dst;
+        uint32_t piece = at, t = 0;
         while (piece >= pools.pieces[t]) piece -= pools.pieces[t++];
-        const uint32_t src = from[pair], dst = to[pair];
+        pair += pairs_on;
+        at += pieces_on;
+        if (at >= pools.pieces_all) {
+            at -= pools.pieces_all;
+            ++pair;
+        }
+        if (item + gridDim.x < items) {
+            next_src = from[pair];
+            next_dst = to[pair];
+        }
         if (src >= pool_pages || dst >= pool_pages) {
             if (threadIdx.x == 0) report(d_status, DEV_BAD_PAGE);
             continue;

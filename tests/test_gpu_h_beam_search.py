@@ -360,6 +360,25 @@ def test_bad_parents_and_pages_are_reported():
     assert int(book.status[0]) == 4 and host(book.lengths).tolist() == [5, 1, 3, 9]
 
 
+@pytest.mark.parametrize("sequences", [4096, 4097, 12288])
+def test_the_largest_books_fork(sequences):
+    book = Book(sequences, 3, 2, 2 * sequences + 7)
+    rng = np.random.default_rng(sequences)
+    book.reserve([int(r) for r in rng.integers(0, 4, sequences)])
+    book.fork([int(p) for p in rng.integers(0, sequences, sequences)])
+    book.check()
+
+
+def test_a_row_alone_stays_and_its_bad_parent_is_reported():
+    t = torch.arange(3 * 8, dtype=torch.int32, device="cuda").view(3, 8)
+    for parents, want in (([0, 1, 2], 0), ([0, 2, 2], 6)):
+        status = status_word()
+        one, size = (C.c_void_p * 1)(t.data_ptr()), (C.c_uint64 * 1)(32)
+        ok(lib().tnsr_b200_reorder_states(one, size, size, 1, ptr(u32(parents)), 3, 1, ptr(status), stream()))
+        torch.cuda.synchronize()
+        assert int(status[0]) == want and t.flatten().tolist() == list(range(24))
+
+
 def test_pages_are_copied_onto_others():
     book = Book(1, 1, 1, 50, (16, 33, 70000))
     pairs = [(3, 7), (9, 8), (3, 49), (0, 1)]

@@ -119,9 +119,10 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(PageBook b, const uint3
 
 int launch_pages_fork(const PageBook& b, const uint32_t* parents, cudaStream_t stream) {
     if (b.sequences == 0) return TNSR_B200_OK;
-    // at most 48 KB of shared memory; few sequences: two columns a block, for less to do one thing behind the other
+    // Columns of a block: with few sequences two, for less to do one thing behind the other; with more than 48 KB of them fewer, down to one: 12 bytes a sequence
     uint32_t columns = b.sequences > 256 ? 8 : 2;
     while (columns > 1 && (uint64_t)(columns + 2) * b.sequences > 12288) columns /= 2;
+    if (int rc = allow_shared<pages_fork_kernel>(3 * PAGES_MAX_SEQUENCES * 4, "pages_fork attribute")) return rc;
     const PageScratch ws = page_scratch(b.workspace, b.sequences, b.pool_pages);
     launch_kernel(pages_fork_kernel, dim3(ceil_div(b.table_ld, columns)), dim3(256), (size_t)(columns + 2) * b.sequences * 4, stream, b, parents, columns,
                   ws.header + 1);
@@ -549,7 +550,7 @@ static void launch_reorder(const StateList& list, uint32_t count, uint64_t most,
 
 int launch_reorder_states(void* const* tensors, const uint64_t* row_bytes, const uint64_t* pitches, uint32_t count, const uint32_t* parents,
                           uint32_t groups, uint32_t beams, int* d_status, cudaStream_t stream) {
-    if (groups == 0 || beams <= 1) return TNSR_B200_OK;
+    if (groups == 0 || (beams == 1 && !d_status)) return TNSR_B200_OK;        // a row alone stays; a parent outside is still told
     for (uint32_t first = 0; first < count; first += RO_TENSORS) {
         const uint32_t n = std::min(count - first, RO_TENSORS);
         uint64_t bits = 0, most = 0;

@@ -824,6 +824,7 @@ TNSR_B200_API int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, 
  * in i's group (rows group * beams .. group * beams + beams - 1; beams <= 32), else row i stays and the status word says
  * 6.  Tensor t: rows of row_bytes[t] bytes, pitches[t] bytes apart (so that of a
  * contiguous cache [sequences, capacity, width] the live prefix alone can move).
+ * No two rows may share bytes, of one tensor or of two.
  * parents: device memory, as beam_select wrote them. */
 TNSR_B200_API int tnsr_b200_reorder_states(void* const* tensors, const uint64_t* row_bytes, const uint64_t* pitches, uint32_t count,
                                            const uint32_t* parents, uint32_t groups, uint32_t beams, int* d_status, void* stream);
@@ -897,7 +898,8 @@ TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args
  * keys that the row sees.  Rows, strides and lengths as for paged_append: row i of n
  * is at position p = lengths[s] - n + i and sees j <= p; with window > 0 those with
  * j > p - window and, beside them, j < sinks.  Pages that no row sees are not
- * looked at.  A row that sees nothing (lengths[s] < n) gives zeros; rows of no
+ * looked at.  A row that sees nothing (lengths[s] < n), or nothing but scores of
+ * -inf, gives zeros; rows of no
  * sequence are left as they were.  q [rows, heads, dim] with q_ld and out
  * [rows, heads, vdim] with out_ld elements between rows; head h reads key/value
  * head h / (heads / kv_heads).  dim, vdim <= 256.  Scores, maxima, sums and

@@ -141,7 +141,7 @@ class Cache:
                     spread = w @ vs[:, h // per].abs()
                     # a score is off by its product's rounding (dim + 8 steps of f32 of the sum of magnitudes), and with it every weight, above and below;
                     # sums of weights and of weighted values by a step per key; an exponential by 2^-20 at the most
-                    magnitude = float((self.scale * (ks[:, h // per].abs() @ q.abs())).max())
+                    magnitude = float((abs(self.scale) * (ks[:, h // per].abs() @ q.abs())).max())
                     rel = 4 * (self.dim + 8) * 2.0 ** -24 * magnitude + 2 * len(ks) * 2.0 ** -24 + 2.0 ** -20
                     if self.dtype == "bf16":
                         # weights in the value product: bf16 (half a step, 2^-8); the result is rounded once (2^-8 of it and of what it is off by)

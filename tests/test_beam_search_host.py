@@ -116,6 +116,7 @@ def test_rows_over_pages_refuse(library, make, entry):
         refuses(call(C.byref(make(**{name: 0})), None), "positive")
     refuses(call(C.byref(make(dtype=2)), None), "dtype")
     refuses(call(C.byref(make(rows=3)), None), "row_starts")
+    refuses(call(C.byref(make(kv_heads=1 << 26)), None), "2^31")
     refuses(call(C.byref(make(rows=1 << 31, row_starts=SOME)), None), "rows")
     assert call(C.byref(make(rows=0, sequences=0)), None) == 0
     if make is append:

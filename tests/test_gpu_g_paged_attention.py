@@ -66,6 +66,26 @@ def test_long_prompts(window, sinks):
     cache.check(cache.run())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [7, 2, 11], [140, 60, 40]])
+def test_windows_as_long_as_a_sequence_or_longer_than_any_position(counts, dtype):
+    cache = Cache([210, 100, 77], counts, 4, 2, 64, 64, 16, dtype, seed=12)
+    want = cache.run()
+    cache.check(want)
+    for window, sinks in ((211, 0), (256, 5), (0x7fffffff, 1), (0x80000000, 0), (0x80000003, 0xffffffff), (NONE, 3)):
+        assert torch.equal(cache.run(window=window, sinks=sinks), want) or window == 211, window
+        cache.check(cache.run(window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30])
+@pytest.mark.parametrize("shape", [(4, 2, 64, 64, 16), (2, 1, 160, 160, 16), (2, 2, 7, 9, 5)])
+def test_scales_of_zero_and_below(shape, scale, dtype):
+    cache = Cache([210, 100, 3], [70, 1, 5], *shape, dtype, seed=13)
+    cache.scale = scale
+    cache.check(cache.run())
+
+
 def test_prompts_in_32_bits():
     cache = Cache([200, 129, 300], [200, 100, 31], 4, 2, 64, 64, 16, "f32", seed=1, window=50, sinks=2)
     cache.check(cache.run())

@@ -45,6 +45,7 @@ const char* paged_problem(const Args* args, Args& a) {
     if (a.chunk == 0 || a.kv_heads == 0 || a.dim == 0 || a.vdim == 0 || a.table_ld == 0 || a.page_rows == 0 || a.pool_pages == 0 ||
         a.page_rows > PAGED_MAX_KEYS)
         return "sizes must be positive";
+    if ((uint64_t)a.kv_heads * ((uint64_t)a.dim + a.vdim) > 0x7fffffffu) return "rows of more than 2^31 values";
     if (!a.row_starts && (uint64_t)a.sequences * a.chunk != a.rows) return "rows must be sequences * chunk without row_starts";
     if (a.rows > 0x7fffffffu) return "too many rows";
     auto fill = [&](uint64_t& page, uint64_t& row, uint64_t& head, uint32_t width) {
@@ -461,7 +462,7 @@ int tnsr_b200_paged_attention(const tnsr_b200_paged_attention_args* args, void* 
     tnsr_b200_paged_attention_args a;
     if (const char* problem = paged_problem(args, a)) return bad_pages("paged_attention", problem);
     if (!a.q || !a.out) return bad("paged_attention: null pointer");
-    if (a.heads == 0 || a.heads % a.kv_heads || a.q_ld < (uint64_t)a.heads * a.dim || a.out_ld < (uint64_t)a.heads * a.vdim)
+    if (a.heads == 0 || a.heads > 0x7fffffffu || a.heads % a.kv_heads || a.q_ld < (uint64_t)a.heads * a.dim || a.out_ld < (uint64_t)a.heads * a.vdim)
         return bad("paged_attention: kv_heads must divide heads, and rows must hold every head");
     if (a.dim > 256 || a.vdim > 256) {
         set_thread_error("paged_attention: widths are at most 256");

@@ -883,6 +883,7 @@ int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stre
     p.per = fast_div(a.heads / a.kv_heads);
     p.capacity = (uint32_t)std::min<uint64_t>((uint64_t)a.table_ld * a.page_rows, PAGED_MAX_KEYS);
     p.scale_log2 = a.scale * 1.4426950408889634f;
+    if (a.window >= p.capacity) p.a.window = p.a.sinks = 0;          // as long as any sequence; smaller ones are positions, of 31 bits
     // the other kernels copy 16 bytes at a time, and write pairs of columns
     const uint32_t per = dtype == TNSR_B200_F32 ? 4 : 8;
     const uint64_t strides = (uint64_t)a.dim | a.vdim | a.k_page | a.k_row | a.k_head | a.v_page | a.v_row | a.v_head;

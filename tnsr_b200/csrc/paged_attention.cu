@@ -222,87 +222,81 @@ constexpr uint32_t FEW_BLOCKS = 592;             // at the most
 constexpr uint32_t FEW_COUNTERS = 4096;          // bytes before the partial results
 static_assert(FEW_COUNTERS >= FEW_BLOCKS * 4, "a counter per block");
 
-// Partial results of a unit joined by the block that comes last, in the order of the runs.  Layout [block][whether the unit begins in its run][16][W + 2].
-template <int W, typename T>
-__device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
-    __shared__ uint32_t s_last;
-    const uint32_t c0 = (uint32_t)few_div(unit_at, run.length), c1 = (uint32_t)few_div(unit_at + u.tiles - 1, run.length), parts = c1 - c0 + 1;
-    few_sync();
-    if (threadIdx.x == 0) {
-        __threadfence();             // with the barriers before and behind it, for all of the block
-        s_last = atomicAdd(done + c0, 1u) + 1 == parts;
-        if (s_last) done[c0] = 0;
-        __threadfence();
-    }
-    few_sync();
-    if (!s_last) return;
-    // a warp has up to four rows, whose loads are on their way together; lanes hold the factors of 32 parts at a time
+// The rows warp + 4 k of a unit from its `parts` partial results, the first of them at `begin` (there the unit begins in the run), the others at `rest` and behind.
+// What bounds it is the way to L2 and back, so loads are on their way together: all maxima and sums (a lane a part), and beside them the numerators of the
+// first PARTS parts.
+template <int W, int ROWS, typename T>
+__device__ __forceinline__ void few_join_rows(const PagedParams& p, const FewUnit& u, uint32_t parts, const float* begin, const float* rest) {
+    constexpr uint32_t ROW = W + 2, PARTS = 8 / ROWS;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr uint32_t ROW = W + 2;
-    auto part = [&](uint32_t i) { return partial + (((uint64_t)(c0 + i) * 2 + (i == 0)) * 16 + warp) * ROW; };        // row `warp` of it
-    float top[4], sum[4] = {};
-    float2 v[4][W / 64];
+    // what is not there is read as the last of what is, so that no load has a condition
+    auto part = [&](uint32_t i) {
+        i = min(i, parts - 1);
+        return i == 0 ? begin : rest + i * (2 * 16 * ROW);
+    };
+    uint32_t at[ROWS];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        top[k] = -INFINITY;
+    for (int k = 0; k < ROWS; ++k) at[k] = min(warp + 4 * k, u.rows - 1) * ROW;
+    float2 x[PARTS][ROWS][W / 64], v[ROWS][W / 64], st[ROWS];
+    float top[ROWS], sum[ROWS], factor[ROWS];
+    auto load = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+                for (int j = 0; j < W / 64; ++j) x[q][k][j] = __ldcg(reinterpret_cast<const float2*>(part(i + q) + at[k]) + j * 32 + lane);
+    };
+    auto load_st = [&](uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) st[k] = __ldcg(reinterpret_cast<const float2*>(part(i) + at[k] + W));
+    };
+    load_st(lane);
+    load(0);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        top[k] = st[k].x;
+        sum[k] = 0.0f;
 #pragma unroll
         for (int j = 0; j < W / 64; ++j) v[k][j] = make_float2(0.0f, 0.0f);
     }
-    for (uint32_t i = lane; i < parts; i += 32)
+    for (uint32_t i = lane + 32; i < parts; i += 32)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (warp + 4 * k < u.rows) top[k] = fmaxf(top[k], __ldcg(part(i) + 4 * k * ROW + W));
+        for (int k = 0; k < ROWS; ++k) top[k] = fmaxf(top[k], __ldcg(part(i) + at[k] + W));
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int d = 16; d > 0; d /= 2)
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], d));
-    for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
-        const uint32_t n = min(32u, parts - i0);
-        float factor[4] = {};
-        if (lane < n)
+        for (int k = 0; k < ROWS; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], d));
+    for (uint32_t i = 0; i < parts; i += PARTS) {
+        if (i % 32 == 0) {
+            if (i) load_st(i + lane);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (warp + 4 * k < u.rows) {
-                    const float2 x = __ldcg(reinterpret_cast<const float2*>(part(i0 + lane) + 4 * k * ROW + W));
-                    factor[k] = mx_ex2(x.x - (top[k] == -INFINITY ? 0.0f : top[k]));
-                    sum[k] = fmaf(factor[k], x.y, sum[k]);
-                }
-        // eight loads a lane on their way: of a row eight parts, or of four rows two
-        auto add = [&](uint32_t i, auto rows_at_once, auto parts_at_once) {
-            constexpr int ROWS = decltype(rows_at_once)::value, PARTS = decltype(parts_at_once)::value;
-            float2 x[PARTS][ROWS][W / 64];
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-                const float* src = part(i0 + min(i + q, n - 1));
-#pragma unroll
-                for (int k = 0; k < ROWS; ++k)
-#pragma unroll
-                    for (int j = 0; j < W / 64; ++j)
-                        x[q][k][j] = warp + 4 * k < u.rows ? __ldcg(reinterpret_cast<const float2*>(src + 4 * k * ROW) + j * 32 + lane) : make_float2(0.0f, 0.0f);
+            for (int k = 0; k < ROWS; ++k) {
+                factor[k] = mx_ex2(st[k].x - (top[k] == -INFINITY ? 0.0f : top[k]));
+                if (i + lane < parts) sum[k] = fmaf(factor[k], st[k].y, sum[k]);
             }
+        }
+        if (i) load(i);
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q)
+        for (uint32_t q = 0; q < PARTS; ++q)
 #pragma unroll
-                for (int k = 0; k < ROWS; ++k) {
-                    const float f = __shfl_sync(0xffffffffu, factor[k], (i + q) & 31);
-                    if (i + q >= n) continue;
+            for (int k = 0; k < ROWS; ++k) {
+                const float f = __shfl_sync(0xffffffffu, factor[k], (i + q) & 31);
+                if (i + q < parts)
 #pragma unroll
                     for (int j = 0; j < W / 64; ++j) {
                         v[k][j].x = fmaf(f, x[q][k][j].x, v[k][j].x);
                         v[k][j].y = fmaf(f, x[q][k][j].y, v[k][j].y);
                     }
-                }
-        };
-        if (u.rows <= 4)
-            for (uint32_t i = 0; i < n; i += 8) add(i, std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-        else
-            for (uint32_t i = 0; i < n; i += 2) add(i, std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+            }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t r = warp + 4 * k;
+    for (int d = 16; d > 0; d /= 2)
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
+        for (int k = 0; k < ROWS; ++k) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], d);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const uint32_t r = warp + 4 * k;
         if (r >= u.rows) continue;
         const float inv = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
         const uint32_t R = u.row0 + r, token = p.per.div(R), h = u.kvh * p.per.d + R - token * p.per.d;
@@ -314,6 +308,27 @@ __device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u,
             if (c + 1 < p.a.vdim) out[c + 1] = from_f32<T>(v[k][j].y * inv);
         }
     }
+}
+
+// Partial results of a unit joined by the block that comes last, in the order of the runs.  Layout [block][whether the unit begins in its run][16][W + 2].
+template <int W, typename T>
+__device__ __forceinline__ void few_join(const PagedParams& p, const FewUnit& u, uint64_t unit_at, const FewRun& run, const float* partial, uint32_t* done) {
+    __shared__ uint32_t s_last;
+    const uint32_t c0 = (uint32_t)few_div(unit_at, run.length), c1 = (uint32_t)few_div(unit_at + u.tiles - 1, run.length), parts = c1 - c0 + 1;
+    few_sync();
+    if (threadIdx.x == 0) {
+        // releases what the block wrote (the barrier is before it) and acquires what the others did (a barrier is behind it)
+        uint32_t before;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(done + c0) : "memory");
+        s_last = before + 1 == parts;
+        if (s_last) done[c0] = 0;
+    }
+    few_sync();
+    if (!s_last) return;
+    const float *rest = partial + (uint64_t)c0 * 2 * 16 * (W + 2), *begin = rest + 16 * (W + 2);
+    if (u.rows <= 4) few_join_rows<W, 1, T>(p, u, parts, begin, rest);
+    else if (u.rows <= 8) few_join_rows<W, 2, T>(p, u, parts, begin, rest);
+    else few_join_rows<W, 4, T>(p, u, parts, begin, rest);
 }
 
 // Shared memory: STAGES tiles of keys and values, rows in parts of 128 bytes whose 16-byte pieces lie at (piece ^ row % 8), so that neither eight rows of a
@@ -459,7 +474,7 @@ __device__ __forceinline__ bool few_odd_values(const PagedParams& p, const FewUn
 // 64 keys, so that nothing is left to be added up between the warps but the sums of the weights.  Weights enter the value product as two bf16 pieces
 // (16 bits): the kernel waits for memory, not for the tensor cores.  Values that are hidden from some rows of a tile may be infinities or NaN, which a weight
 // of 0 does not keep out: such a tile's product is made key by key for each row.
-// The ring keeps 64 to 192 KB per SM on their way: four tiles at widths of 64 (three blocks per SM), three at 128 (two) and 256 (one).
+// The rings keep 192 KB per SM on their way: four tiles at widths of 64 (three blocks per SM), three at 128 (two) and 256 (one).
 constexpr uint32_t FEW_P_PITCH = 64 * 2 + 16, FEW_P_BYTES = 2 * 16 * FEW_P_PITCH;
 
 template <int W, bool UPPER, bool TMA>
@@ -724,21 +739,20 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
 #pragma unroll
             for (int r = 0; r < RQ * 4; ++r) {
                 if (r >= c.u.rows) continue;
-                const uint32_t R = c.u.row0 + r, token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
-                const float inv = sums[r] == 0.0f ? 0.0f : 1.0f / sums[r];
-                float* out = reinterpret_cast<float*>(a.out) + (uint64_t)(c.u.seq.start + token) * a.out_ld + (uint64_t)h * a.vdim;
                 float* dst = partial + (((uint64_t)blockIdx.x * 2 + (unit_at >= run.begin)) * 16 + r) * (W + 2);
+                float inv = 1.0f;
+                if (all) {
+                    const uint32_t R = c.u.row0 + r, token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
+                    dst = reinterpret_cast<float*>(a.out) + (uint64_t)(c.u.seq.start + token) * a.out_ld + (uint64_t)h * a.vdim;
+                    inv = sums[r] == 0.0f ? 0.0f : 1.0f / sums[r];
+                }
 #pragma unroll
                 for (int n = 0; n < COLUMNS; ++n) {
                     const uint32_t x = col + n * 128;
                     const float v = W == 64 ? o[n][r] + half_sums[r * 64 + col] : o[n][r];
-                    if (!all) dst[x] = v;
-                    else if (x < a.vdim) out[x] = v * inv;
+                    if (!all || x < a.vdim) dst[x] = v * inv;
                 }
-                if (!all && tid == 0) {
-                    dst[W] = tops[r];
-                    dst[W + 1] = sums[r];
-                }
+                if (!all && tid == 0) *reinterpret_cast<float2*>(dst + W) = make_float2(tops[r], sums[r]);
             }
         }
         return all;
@@ -749,19 +763,20 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
         uint8_t* tile = ring.tiles + stage * 2 * S::TILE;
         mbar_wait(ring.full + stage, (n / S::STAGES) & 1, ring.abort_flag, limit);      // given up: the run goes on without waiting
         few_sync();                          // the rows of a new unit are there, the weights of the last tile have been read
-        float dot[RQ] = {};
-#pragma unroll 8
-        for (int x = 0; x < W / 4; ++x) {
+        float dot[RQ] = {}, odd_dot[RQ] = {};
+#pragma unroll 4
+        for (uint32_t x = 0; x < a.dim / 4; ++x) {
             const float4 kv = *reinterpret_cast<const float4*>(tile + S::at(lane, x));
 #pragma unroll
             for (int i = 0; i < RQ; ++i) {
                 const float4 q = reinterpret_cast<const float4*>(sq + (warp + 4 * i) * W)[x];
-                dot[i] = fmaf(q.x, kv.x, fmaf(q.y, kv.y, fmaf(q.z, kv.z, fmaf(q.w, kv.w, dot[i]))));
+                dot[i] = fmaf(q.x, kv.x, fmaf(q.y, kv.y, dot[i]));
+                odd_dot[i] = fmaf(q.z, kv.z, fmaf(q.w, kv.w, odd_dot[i]));
             }
         }
 #pragma unroll
         for (int i = 0; i < RQ; ++i) {
-            const float x = row_sees(p, places[warp + 4 * i], key0 + lane) ? dot[i] : -INFINITY;
+            const float x = row_sees(p, places[warp + 4 * i], key0 + lane) ? dot[i] + odd_dot[i] : -INFINITY;
             float top = fmaxf(m[i], x);
 #pragma unroll
             for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));

@@ -703,12 +703,16 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
         unit_at = c.at - c.tile;
         few_sync();                     // the last unit's rows are done with
         const int32_t base = (int32_t)c.u.seq.length - (int32_t)c.u.seq.count;
-        for (uint32_t i = tid; i < RQ * 4 * W; i += 128) {
-            const uint32_t r = i / W, x = i % W, R = c.u.row0 + min(r, c.u.rows - 1), token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
-            sq[i] = r < c.u.rows && x < a.dim
-                        ? reinterpret_cast<const float*>(a.q)[(uint64_t)(c.u.seq.start + token) * a.q_ld + (uint64_t)h * a.dim + x] * p.scale_log2 : 0.0f;
+        // all loads on their way together
+        float q[RQ * 4 * W / 128];
+#pragma unroll
+        for (uint32_t n = 0; n < RQ * 4 * W / 128; ++n) {
+            const uint32_t i = n * 128 + tid, r = i / W, x = i % W, R = c.u.row0 + min(r, c.u.rows - 1), token = p.per.div(R), h = c.u.kvh * p.per.d + R - token * p.per.d;
+            q[n] = r < c.u.rows && x < a.dim ? reinterpret_cast<const float*>(a.q)[(uint64_t)(c.u.seq.start + token) * a.q_ld + (uint64_t)h * a.dim + x] : 0.0f;
             if (x == 0) places[r] = base + (int32_t)token;
         }
+#pragma unroll
+        for (uint32_t n = 0; n < RQ * 4 * W / 128; ++n) sq[n * 128 + tid] = q[n] * p.scale_log2;
 #pragma unroll
         for (int i = 0; i < RQ * 4; ++i)
 #pragma unroll

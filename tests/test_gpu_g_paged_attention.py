@@ -233,6 +233,83 @@ def test_prompts_behind_one_another_whose_items_have_one_tile_or_two(dim):
             assert torch.equal(c.out[:c.rows].float().cpu(), w)
 
 
+# few prompts over long caches: the last round's keys are divided over the blocks, and a tile's parts joined
+@pytest.mark.parametrize("shape", [(4, 2, 64, 64, 16), (2, 1, 128, 128, 64), (6, 2, 96, 40, 24)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1900, 5), (2047, 300)])
+def test_few_prompts_over_long_caches(shape, window, sinks):
+    cache = Cache([3000, 1700, 50, 2500], [100, 70, 60, 130], *shape, "bf16", seed=window + 2, window=window, sinks=sinks, extra_rows=2)
+    got = cache.run()
+    cache.check(got)
+    assert float((got[-2:] + 7).abs().max()) == 0.0
+    cache = Cache([2600, 40, 130], [150, 150, 150], *shape, "bf16", seed=window + 3, window=window, sinks=sinks, uniform=True)
+    cache.check(cache.run())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_prompts_over_long_caches_hide_what_is_hidden(dim):
+    cache = Cache([3100, 2300], [90, 140], 4, 2, dim, dim, 16, "bf16", seed=8, window=2200, sinks=3)
+    clean = cache.run().clone()
+    table = cache.host_table
+    seen = [[], []]
+    for s, n in enumerate(cache.lengths):
+        first = n - cache.counts[s]                  # position of the first new row: its window begins 2200 keys before
+        for at in (n - 1, n - 30, first - 2200 + 20):
+            if at < 3:
+                continue
+            page, r = int(table[s, at // 16]), at % 16
+            cache.v_pool[page, r, 0, 3], cache.v_pool[page, r, 1, 5] = float("nan"), float("inf")
+            seen[s].append(at)
+    got = cache.run()
+    for s, n in enumerate(cache.lengths):
+        for i in range(cache.counts[s]):
+            row, at = int(cache.starts[s]) + i, n - cache.counts[s] + i
+            sees = any(j <= at and j > at - 2200 for j in seen[s])
+            a, b = got[row].view(4, dim), clean[row].view(4, dim)
+            if not sees:
+                assert torch.equal(a, b), (s, i)
+                continue
+            # a value of NaN, or of infinity (its weight may have become 0, which makes NaN of it)
+            assert bool(torch.isnan(a[:2, 3]).all()) and not bool(torch.isfinite(a[2:, 5]).any()), (s, i)
+            others = [c for c in range(dim) if c not in (3, 5)]
+            assert bool(torch.isfinite(a[:, others]).all()) and float((a[:, others] - b[:, others]).abs().max()) < 0.05
+
+
+def test_few_prompts_over_long_caches_again_in_a_graph_and_behind_single_tokens():
+    cache = Cache([3000, 1700, 50], [100, 70, 60], 8, 2, 128, 128, 16, "bf16", seed=14, window=0)
+    tokens = Cache([700, 90], [1, 1], 8, 2, 128, 128, 16, "bf16", seed=15, uniform=True)
+    work = scratch(lib().tnsr_b200_paged_attention_workspace(128, 128, 1))
+    want, want_tokens = cache.run(work).clone(), tokens.run(work).clone()
+    cache.check(want)
+    tokens.check(want_tokens)
+    graph = torch.cuda.CUDAGraph()
+    args, token_args = cache.args(work), tokens.args(work)
+    with torch.cuda.graph(graph):
+        for _ in range(2):
+            ok(lib().tnsr_b200_paged_attention(C.byref(args), stream()))
+            ok(lib().tnsr_b200_paged_attention(C.byref(token_args), stream()))
+    for _ in range(3):
+        cache.out.fill_(-7.0)
+        tokens.out.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache.out[:cache.rows].float().cpu(), want)
+        assert torch.equal(tokens.out[:tokens.rows].float().cpu(), want_tokens)
+    # the captured call follows its lengths: shorter ones, and back
+    lengths = cache.d_lengths.clone()
+    for smaller in ([1200, 900, 50], [100, 70, 60]):
+        cache.d_lengths.copy_(u32(np.array(smaller)))
+        graph.replay()
+        torch.cuda.synchronize()
+        # all but the rows behind the third sequence's 50 keys, whose places in the pool hold NaN
+        assert int(cache.status[0]) == 0 and bool(torch.isfinite(cache.out[:int(cache.starts[2]) + 50].float()).all())
+    cache.d_lengths.copy_(lengths)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(cache.out[:cache.rows].float().cpu(), want)
+    cache.out.fill_(-7.0)
+    cache.check(cache.run(None))
+
+
 def test_many_sequences_and_one_long_one_beside_short_ones():
     rng = np.random.default_rng(0)
     lengths = list(rng.integers(0, 40, 700)) + [5000]

@@ -52,7 +52,9 @@ struct PagedParams {
 
 int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stream);
 uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype);
+constexpr uint32_t PAGED_COUNTERS = 4096;           // bytes of a workspace before its partial results
 // Many rows, on the tensor cores of the fifth generation (paged_prompt.cu).
+uint64_t paged_prompt_workspace_bytes(uint32_t dim, uint32_t vdim);
 bool paged_prompt_eligible(const PagedAttention& a, int dtype);
 int launch_paged_prompt(const PagedParams& p, cudaStream_t stream);
 

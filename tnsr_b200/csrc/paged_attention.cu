@@ -219,8 +219,7 @@ __device__ __forceinline__ bool unit_sees(const PagedParams& p, const FewUnit& u
 }
 
 constexpr uint32_t FEW_BLOCKS = 592;             // at the most
-constexpr uint32_t FEW_COUNTERS = 4096;          // bytes before the partial results
-static_assert(FEW_COUNTERS >= FEW_BLOCKS * 4, "a counter per block");
+static_assert(PAGED_COUNTERS >= FEW_BLOCKS * 4, "a counter per block");
 
 // The rows warp + 4 k of a unit from its `parts` partial results, the first of them at `begin` (there the unit begins in the run), the others at `rest` and behind.
 // What bounds it is the way to L2 and back, so loads are on their way together: all maxima and sums (a lane a part), and beside them the numerators of the
@@ -868,7 +867,7 @@ int launch_few(const PagedParams& p, const FewLaunch& f, cudaStream_t stream) {
     uint32_t* done = nullptr;
     if (p.a.workspace) {
         done = reinterpret_cast<uint32_t*>(p.a.workspace);
-        partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + FEW_COUNTERS);
+        partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.a.workspace) + PAGED_COUNTERS);
     }
     launch_kernel(KERNEL, dim3(f.grid), dim3(160), bytes, stream, f.k, f.v, p, f.box, partial, done, g_wait_limit_ns.load(std::memory_order_relaxed));
     return TNSR_B200_OK;
@@ -891,7 +890,8 @@ int launch_few_any(const PagedParams& p, int dtype, uint32_t width, uint32_t row
 
 uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype) {
     const uint32_t w = few_width(dim, vdim);
-    return FEW_COUNTERS + (uint64_t)few_blocks(w) * 2 * 16 * (w + 2) * 4;
+    const uint64_t few = PAGED_COUNTERS + (uint64_t)few_blocks(w) * 2 * 16 * (w + 2) * 4;
+    return dtype == TNSR_B200_BF16 ? std::max(few, paged_prompt_workspace_bytes(dim, vdim)) : few;
 }
 
 int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stream) {

@@ -14,6 +14,11 @@
 //                 grown by more than 2^8 since the last time (weights then are at most 2^8, sums f32); S of block j is complete only when
 //                 P V of block j - 1 is, so the rescaling needs no barrier of its own.
 //
+// Items go round the grid, the last tokens of every sequence first (they have the most keys).  Those of the last round, fewer than blocks of the grid, are divided
+// where that pays: their key blocks, one item behind the other, are cut into equal runs, a run per block of the grid.  An item whose blocks lie in several
+// runs leaves per run what its rows have so far (maximum, sum, numerators in f32); the run whose part of a tile is written last joins them in the order of
+// the runs.  Every block finds its items by itself from the lengths, so a captured call follows them.
+//
 // Values that some rows of an item see and others do not may hold infinities or NaN, which a weight of 0 does not keep out, and so may the
 // rest of a last page: in blocks that are not seen by all, each row of values is looked through and such elements are zeroed before the
 // product; rows that see one of them are computed once more key by key.
@@ -35,8 +40,12 @@ template <int W>
 struct PromptShape {
     static constexpr uint32_t TILE = PP_HALF * (W / 64);                // 128 rows of W
     static constexpr uint32_t STAGES = W == 128 ? 2 : 4;
-    static constexpr uint32_t BYTES = 1024 + 2 * TILE + STAGES * 2 * TILE + 1024;
+    static constexpr uint32_t PLAN = 2 * TILE + STAGES * 2 * TILE + 1024, BYTES = 1024 + PLAN;      // alignment; tiles, barriers; the plan behind them
 };
+constexpr uint32_t PP_BLOCKS = 148;                  // of the grid: one of an SM
+constexpr uint32_t PP_ENTRIES = 4096;                // pairs of tiles (of all sequences) up to which the last round is divided: the list is in shared memory
+constexpr uint32_t PP_PARTS = 4;                     // that the longest item of the last round is cut into, at the most (and one more where runs begin inside)
+constexpr uint32_t PP_JOIN = 8;                      // key blocks that could be gone through in the time that a join takes
 constexpr uint32_t PP_TMEM = 512;                    // scores 2 x 128, outputs 2 x W
 constexpr uint32_t PP_O = 256;
 
@@ -48,8 +57,11 @@ struct PromptParams {
     PagedParams p;
     uint32_t tokens;             // of a tile
     uint32_t pairs;              // items of a sequence and key/value head at the most
+    uint32_t units, items;       // sequences x key/value heads; items if all are there
     uint32_t box;                // rows of a key box
     uint64_t wait_limit_ns;
+    float* partial;              // divided: [block][whether the item begins in its run][2 tiles][W + 2][128 rows]; else null
+    uint32_t* done;              // [block][2 tiles], zero between launches
 };
 
 // Matrix descriptors differ in their lower word only, by constants: one thread issues all products of the block, and what it computes
@@ -143,14 +155,12 @@ __device__ __forceinline__ bool partly_seen(const PagedParams& p, const PromptIt
     return (int32_t)key0 + 127 > it.first[t0] || ((int32_t)key0 < it.whole[t1] && key0 + 128 > p.a.sinks);
 }
 
-// Items in the order in which blocks of the grid take them: of every sequence and head the last tokens first (they have the most keys).
-__device__ __forceinline__ bool prompt_item(const PromptParams& prm, uint64_t index, PromptItem& it) {
+// Tiles 2 pair and 2 pair + 1 of a sequence and key/value head; false: there are no such rows.
+__device__ __forceinline__ bool prompt_item(const PromptParams& prm, uint32_t s, uint32_t kvh, uint32_t pair, PromptItem& it) {
     const PagedParams& p = prm.p;
-    const uint32_t units = p.a.sequences * p.a.kv_heads, rest = (uint32_t)(index % units);
-    it.s = rest / p.a.kv_heads;
-    it.kvh = rest % p.a.kv_heads;
+    it.s = s;
+    it.kvh = kvh;
     it.seq = paged_sequence(p, it.s);
-    const uint32_t pair = prm.pairs - 1 - (uint32_t)(index / units);
     it.token0 = pair * 2 * prm.tokens;
     if (it.token0 >= it.seq.count) return false;
     const uint32_t left = it.seq.count - it.token0;
@@ -175,12 +185,137 @@ __device__ __forceinline__ bool prompt_item(const PromptParams& prm, uint64_t in
     it.blocks = it.head_blocks + (uint32_t)it.high / 128 - it.gap + 1;
     return true;
 }
-// Blocks up to the last one that a tile sees.
-__device__ __forceinline__ uint32_t tile_blocks(const PromptItem& it, int t) {
-    return it.last[t] < 0 ? 0u : it.head_blocks + (uint32_t)it.last[t] / 128 - it.gap + 1;
+// The last block of [j0, j1) that a tile sees, + 1; 0: none.
+__device__ __forceinline__ uint32_t last_seen(const PagedParams& p, const PromptItem& it, int t, uint32_t j0, uint32_t j1) {
+    uint32_t j = it.last[t] < 0 ? 0u : it.head_blocks + (uint32_t)it.last[t] / 128 - it.gap + 1;
+    if (j0 == 0 && j1 == it.blocks) return j;
+    j = min(j, j1);
+    while (j > j0 && !tile_sees(p, it, t, item_key0(it, j - 1))) --j;
+    return j > j0 ? j : 0u;
+}
+// In shared memory: which items there are, and what becomes of the last round's.
+struct PromptPlan {
+    uint32_t whole;                  // items below this number are taken whole, every gridDim.x-th one
+    uint32_t divided;                // number of the first item of the last round
+    uint32_t first, length, end;     // the block's run: its first item (of the last round), key blocks of a run, where it ends
+    uint32_t most;                   // key blocks of the longest of them
+    uint32_t before[PP_BLOCKS];      // key blocks before an item of the last round
+    uint32_t entries[PP_ENTRIES];    // pairs of tiles that are there: (pairs - 1 - pair) * sequences + sequence
+};
+
+// A block's way through the work.  Undivided: items by number, those that are not there passed over.
+template <bool DIVIDED>
+struct PromptWalk {
+    uint32_t next;
+    __device__ __forceinline__ PromptWalk(const PromptPlan&) : next(blockIdx.x) {}
+    // key blocks of the item that are this block's
+    __device__ __forceinline__ uint32_t begin() const { return 0; }
+    __device__ __forceinline__ uint32_t end(const PromptItem& it) const { return it.blocks; }
+    __device__ __forceinline__ bool more(const PromptParams& prm, const PromptPlan&) const { return next < prm.items; }
+    __device__ __forceinline__ bool step(const PromptParams& prm, const PromptPlan&, PromptItem& it) {
+        const uint32_t row = next / prm.units, rest = next - row * prm.units;
+        next += gridDim.x;
+        return prompt_item(prm, rest / prm.p.a.kv_heads, rest % prm.p.a.kv_heads, prm.pairs - 1 - row, it);
+    }
+};
+// Divided: whole items by their number among those that are there, then the run.
+template <>
+struct PromptWalk<true> {
+    uint32_t number, at;             // whole items: the next one; then the next key block of the run
+    uint32_t j0, j1;
+    __device__ __forceinline__ uint32_t begin() const { return j0; }
+    __device__ __forceinline__ uint32_t end(const PromptItem& it) const { return it.blocks ? j1 : 0u; }
+    __device__ __forceinline__ PromptWalk(const PromptPlan& plan) : number(blockIdx.x), at(plan.length * blockIdx.x), j0(0), j1(0) {}
+    __device__ __forceinline__ bool more(const PromptParams&, const PromptPlan& plan) const { return number < plan.whole || at < plan.end; }
+    // the next item; false: it is not there
+    __device__ __forceinline__ bool step(const PromptParams& prm, const PromptPlan& plan, PromptItem& it) {
+        const PagedParams& p = prm.p;
+        if (number >= plan.whole) {
+            if (at == plan.length * blockIdx.x) number = plan.divided + plan.first;
+        }
+        const uint32_t entry = number / p.a.kv_heads, e = plan.entries[entry], row = e / p.a.sequences;
+        prompt_item(prm, e - row * p.a.sequences, number - entry * p.a.kv_heads, prm.pairs - 1 - row, it);
+        j0 = 0;
+        j1 = it.blocks;
+        if (number < plan.whole) {
+            number += gridDim.x;
+            return true;
+        }
+        const uint32_t begin = plan.before[number - plan.divided];
+        j0 = at - begin;
+        j1 = min(max(it.blocks, 1u), plan.end - begin);
+        at = begin + j1;
+        ++number;
+        return true;
+    }
+};
+
+// Exclusive prefix sum over the block.
+__device__ __forceinline__ uint32_t prompt_scan(uint32_t v, uint32_t* warps, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) warps[warp] = x;
+    __syncthreads();
+    uint32_t before = x - v;
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < PP_THREADS / 32; ++w) {
+        if (w < warp) before += warps[w];
+        total += warps[w];
+    }
+    __syncthreads();
+    return before;
 }
 
-template <int W>
+// Which items there are, and this block's run of those of the last round.
+__device__ __forceinline__ void prompt_plan(const PromptParams& prm, PromptPlan& plan, uint32_t* warps) {
+    const PagedParams& p = prm.p;
+    const uint32_t all = p.a.sequences * prm.pairs, share = (all + PP_THREADS - 1) / PP_THREADS;
+    const uint32_t e0 = min(all, threadIdx.x * share), e1 = min(all, e0 + share);
+    PromptItem it;
+    uint32_t total = all;
+    if (p.a.row_starts) {
+        uint32_t mine = 0;
+        for (uint32_t e = e0; e < e1; ++e) mine += prompt_item(prm, e % p.a.sequences, 0, prm.pairs - 1 - e / p.a.sequences, it);
+        uint32_t at = prompt_scan(mine, warps, total);
+        for (uint32_t e = e0; e < e1; ++e)
+            if (prompt_item(prm, e % p.a.sequences, 0, prm.pairs - 1 - e / p.a.sequences, it)) plan.entries[at++] = e;
+    } else {
+        for (uint32_t e = threadIdx.x; e < all; e += PP_THREADS) plan.entries[e] = e;
+    }
+    if (threadIdx.x == 0) plan.most = 0;
+    __syncthreads();
+    const uint32_t items = total * p.a.kv_heads, left = items % gridDim.x, divided = items - left;
+    uint32_t weight = 0, blocks;
+    if (threadIdx.x < left) {
+        const uint32_t number = divided + threadIdx.x, e = plan.entries[number / p.a.kv_heads];
+        prompt_item(prm, e % p.a.sequences, 0, prm.pairs - 1 - e / p.a.sequences, it);
+        weight = max(it.blocks, 1u);                  // rows that see nothing become zeros
+        atomicMax(&plan.most, weight);
+    }
+    const uint32_t before = prompt_scan(weight, warps, blocks);
+    // a join reads all parts: no more than some of an item
+    const uint32_t length = max((plan.most + PP_PARTS - 1) / PP_PARTS, (blocks + gridDim.x - 1) / gridDim.x), begin = length * blockIdx.x;
+    const bool pays = plan.most > length + PP_JOIN;
+    if (threadIdx.x < left) {
+        plan.before[threadIdx.x] = before;
+        if (begin >= before && begin < before + weight) plan.first = threadIdx.x;
+    }
+    if (threadIdx.x == 0) {
+        plan.length = length;
+        plan.divided = divided;
+        plan.whole = pays ? divided : items;
+        plan.end = pays ? min(begin + length, blocks) : 0u;
+    }
+    __syncthreads();
+}
+
+template <int W, bool DIVIDED>
 __global__ void __launch_bounds__(PP_THREADS, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ PromptParams prm) {
@@ -224,6 +359,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     pdl_wait();
     pdl_trigger();
+    __shared__ volatile uint32_t join_now[2];
+    PromptPlan& plan = *reinterpret_cast<PromptPlan*>(smem + S::PLAN);
+    if constexpr (DIVIDED) {
+        __shared__ uint32_t warps[PP_THREADS / 32];
+        prompt_plan(prm, plan, warps);
+    }
+    PromptWalk<DIVIDED> walk(plan);
     if (warp == 1) {
         tmem_alloc(tmem_slot, PP_TMEM);
         tmem_relinquish();
@@ -232,7 +374,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint64_t items = (uint64_t)p.a.sequences * p.a.kv_heads * prm.pairs;
     PromptItem it;
 
     auto teardown = [&]() {
@@ -258,10 +399,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         // ---------------- copies ----------------
         uint32_t blocks = 0, used[2] = {0, 0};       // key blocks so far; items so far that had rows in a tile
         bool ok = true;
-        for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
-            if (!prompt_item(prm, index, it) || it.blocks == 0) continue;
+        while (ok && walk.more(prm, plan)) {
+            if (!walk.step(prm, plan, it) || it.blocks == 0) continue;
             const uint32_t boxes = 128 / prm.box;
-            for (uint32_t j = 0; ok && j < it.blocks; ++j, ++blocks) {
+            const uint32_t j0 = walk.begin(), j1 = walk.end(it);
+            for (uint32_t j = j0; ok && j < j1; ++j, ++blocks) {
                 const uint32_t stage = blocks % STAGES, parity = ((blocks / STAGES) & 1) ^ 1;
                 const uint32_t key = item_key0(it, j) + lane * prm.box;
                 int32_t page = (int32_t)p.a.pool_pages, row = 0;          // outside: zeros
@@ -281,7 +423,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (uint32_t h = 0; h < HALVES; ++h)
                         tma_load_4d(smem_u32(k_ring) + stage * S::TILE + h * PP_HALF + lane * prm.box * 128, &map_k, (int32_t)(h * 64), (int32_t)it.kvh, row, page,
                                    k_full + stage);
-                if (j == 0) {
+                if (j == j0) {
                     for (int t = 0; t < 2 && ok; ++t) {
                         if (!it.tokens[t]) continue;
                         ok = used[t] == 0 || mbar_wait(q_empty + t, (used[t] - 1) & 1, abort_flag, limit);
@@ -328,11 +470,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 umma_commit(s_full + t);
             };
             bool ok = true;
-            for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
-                if (!prompt_item(prm, index, it) || it.blocks == 0) continue;
+            while (ok && walk.more(prm, plan)) {
+                if (!walk.step(prm, plan, it) || it.blocks == 0) continue;
+                const uint32_t j0 = walk.begin(), j1 = walk.end(it);
                 // behind the scores of the last block that a tile sees its queries may change, behind its product the output is complete; a tile
                 // that sees nothing gives its queries back with the item's first block
-                const uint32_t last[2] = {tile_blocks(it, 0), tile_blocks(it, 1)};
+                const uint32_t last[2] = {last_seen(p, it, 0, j0, j1), last_seen(p, it, 1, j0, j1)};
                 uint32_t accumulate[2] = {0, 0};
                 for (int t = 0; t < 2 && ok; ++t)
                     if (it.tokens[t]) {
@@ -342,17 +485,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (!ok) break;
                 auto scores = [&](uint32_t j, int t, bool sees, uint32_t stage) {
                     if (sees) issue_s(t, stage);
-                    if (it.tokens[t] && j + 1 == max(last[t], 1u)) umma_commit(q_empty + t);
+                    if (it.tokens[t] && j + 1 == max(last[t], j0 + 1)) umma_commit(q_empty + t);
                 };
-                uint32_t stage = blocks % STAGES, parity = (blocks / STAGES) & 1, key0 = item_key0(it, 0);
+                uint32_t stage = blocks % STAGES, parity = (blocks / STAGES) & 1, key0 = item_key0(it, j0);
                 bool sees[2] = {tile_sees(p, it, 0, key0), tile_sees(p, it, 1, key0)};
                 if (!mbar_wait(k_full + stage, parity, abort_flag, limit)) break;
                 tc_fence_after();
-                scores(0, 0, sees[0], stage);
-                scores(0, 1, sees[1], stage);
+                scores(j0, 0, sees[0], stage);
+                scores(j0, 1, sees[1], stage);
                 umma_commit(k_empty + stage);
-                for (uint32_t j = 0; j < it.blocks; ++j) {
-                    const bool more = j + 1 < it.blocks;
+                for (uint32_t j = j0; j < j1; ++j) {
+                    const bool more = j + 1 < j1;
                     const uint32_t next = stage + 1 == STAGES ? 0 : stage + 1, next_parity = next ? parity : parity ^ 1;
                     bool then[2] = {false, false};
                     if (more) {
@@ -388,7 +531,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     stage = next;
                     parity = next_parity;
                 }
-                blocks += it.blocks;
+                blocks += j1 - j0;
             }
         }
     }
@@ -402,14 +545,15 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t s_addr = tmem + t * 128 + ((quarter * 32u) << 16), o_addr = tmem + PP_O + t * W + ((quarter * 32u) << 16);
         const uint32_t my_token = p.per.div(row), my_head = row - my_token * p.per.d;
-        uint32_t blocks = 0, seen = 0, outputs = 0, number = 0;      // key blocks; blocks of the tile; outputs; items so far
+        uint32_t blocks = 0, seen = 0, outputs = 0, number = 0, looks = 0;      // key blocks; blocks of the tile; outputs; items; turns of `looked` so far
         bool ok = true;
         // a warp gives up as a whole
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
-        for (uint64_t index = blockIdx.x; ok && index < items; index += gridDim.x) {
-            if (!prompt_item(prm, index, it)) continue;
+        while (ok && walk.more(prm, plan)) {
+            if (!walk.step(prm, plan, it)) continue;
+            const uint32_t j0 = walk.begin(), j1 = walk.end(it);
             if (!it.tokens[t]) {
-                blocks += it.blocks;
+                blocks += j1 - j0;
                 continue;
             }
             const int32_t at = it.first[t] + (int32_t)min(my_token, it.tokens[t] - 1);
@@ -417,8 +561,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
             float m = -INFINITY, l = 0.0f;
             bool any = false;
-            for (uint32_t j = 0; j < it.blocks; ++j) {
-                const uint32_t b = blocks + j, key0 = item_key0(it, j);
+            for (uint32_t j = j0; j < j1; ++j) {
+                const uint32_t b = blocks + (j - j0), key0 = item_key0(it, j);
                 if (!tile_sees(p, it, t, key0)) continue;
                 any = true;
                 if (!wait(s_full + t, seen & 1)) { ok = false; break; }
@@ -531,7 +675,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + t);
             }
-            blocks += it.blocks;
+            blocks += j1 - j0;
             if (!ok) break;
             if (any) {
                 if (!wait(o_full + t, outputs & 1)) { ok = false; break; }
@@ -541,7 +685,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // whether the row sees something that must not be multiplied by 0 (a warp that is ahead writes to the other place)
             __syncwarp();
             if (lane == 0) mbar_arrive(looked + t);
-            if (!wait(looked + t, (number - 1) & 1)) { ok = false; break; }
+            if (!wait(looked + t, (DIVIDED ? looks++ : number - 1) & 1)) { ok = false; break; }
             bool mine = my_token < it.tokens[t], odd = false;
             const uint32_t slot = 2 * t + (number & 1), found = *(volatile uint32_t*)(odd_seen + slot);
             if (found >> 8 == number) {
@@ -553,34 +697,108 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 odd &= mine;
                 mine &= !odd;
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bf16* out = reinterpret_cast<bf16*>(p.a.out) + (uint64_t)(it.seq.start + it.token0 + t * prm.tokens + my_token) * p.a.out_ld +
                         (uint64_t)(it.kvh * p.per.d + my_head) * p.a.vdim;
+            bool joined = false;                     // or left to be
+            if constexpr (DIVIDED) {
+                joined = j0 != 0 || j1 < it.blocks;
+                if (joined) {
+                    // in part: the row's maximum (+inf: to be computed once more), sum and numerators
+                    float* dst = prm.partial + (((uint64_t)blockIdx.x * 2 + (j0 == 0)) * 2 + t) * 128 * (W + 2) + row;
 #pragma unroll
-            for (int c = 0; c < W / 16; ++c) {
-                float o[16];
-                if (any) pp_ld16(o_addr + c * 16, o);
+                    for (int c = 0; c < W / 16; ++c) {
+                        float o[16];
+                        if (!any) break;
+                        pp_ld16(o_addr + c * 16, o);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (!mine || (uint32_t)(c * 16 + i * 8) >= p.a.vdim) continue;
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (l != 0.0f) {
-                        w.x = pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv);
-                        w.y = pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
-                        w.z = pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
-                        w.w = pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+                        for (int i = 0; i < 16; ++i) dst[(c * 16 + i) * 128] = o[i];
                     }
-                    *reinterpret_cast<uint4*>(out + c * 16 + i * 8) = w;
+                    dst[W * 128] = odd ? INFINITY : m * p.scale_log2;
+                    dst[(W + 1) * 128] = l;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(looked + t);
+                    if (!wait(looked + t, looks++ & 1)) { ok = false; break; }
+                    const uint32_t item_at = plan.before[walk.number - 1 - plan.divided], c0 = item_at / plan.length,
+                                   parts = (item_at + it.blocks - 1) / plan.length - c0 + 1;
+                    if (row == 0) {
+                        __threadfence();             // with the barriers before and behind it, for all of the tile
+                        const bool last = atomicAdd(prm.done + c0 * 2 + t, 1u) + 1 == parts;
+                        if (last) prm.done[c0 * 2 + t] = 0;
+                        __threadfence();
+                        join_now[t] = last;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(looked + t);
+                    if (!wait(looked + t, looks++ & 1)) { ok = false; break; }
+                    if (!join_now[t]) continue;
+                    const bool there = my_token < it.tokens[t];
+                    const float* tile = prm.partial + ((uint64_t)c0 * 4 + t) * 128 * (W + 2) + row;
+                    auto part = [&](uint32_t i) {
+                        i = min(i, parts - 1);
+                        return tile + ((uint64_t)i * 2 + (i == 0)) * 2 * 128 * (W + 2);
+                    };
+                    float factor[PP_PARTS + 1], top = -INFINITY, sum = 0.0f;
+                    bool known[PP_PARTS + 1];                 // the row saw something in the part: else there is no more of it than its maximum
+#pragma unroll
+                    for (uint32_t i = 0; i <= PP_PARTS; ++i) {
+                        factor[i] = __ldcg(part(i) + W * 128);
+                        top = fmaxf(top, factor[i]);
+                    }
+                    odd = there && top == INFINITY;
+                    const float ms = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                    for (uint32_t i = 0; i <= PP_PARTS; ++i) {
+                        known[i] = i < parts && factor[i] != -INFINITY;
+                        factor[i] = mx_ex2(factor[i] - ms);
+                        if (i < parts) sum = fmaf(factor[i], __ldcg(part(i) + (W + 1) * 128), sum);
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    for (uint32_t c = 0; c < p.a.vdim; c += 8) {
+                        float x[PP_PARTS + 1][8], acc[8] = {};
+#pragma unroll
+                        for (uint32_t i = 0; i <= PP_PARTS; ++i)
+#pragma unroll
+                            for (uint32_t k = 0; k < 8; ++k) x[i][k] = __ldcg(part(i) + (c + k) * 128);
+#pragma unroll
+                        for (uint32_t i = 0; i <= PP_PARTS; ++i)
+                            if (known[i])
+#pragma unroll
+                                for (uint32_t k = 0; k < 8; ++k) acc[k] = fmaf(factor[i], x[i][k], acc[k]);
+                        if (there && !odd)
+                            *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                                                                            pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+                    }
                 }
             }
-            tc_fence_before();
+            if (!joined) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int c = 0; c < W / 16; ++c) {
+                    float o[16];
+                    if (any) pp_ld16(o_addr + c * 16, o);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (!mine || (uint32_t)(c * 16 + i * 8) >= p.a.vdim) continue;
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (l != 0.0f) {
+                            w.x = pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv);
+                            w.y = pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
+                            w.z = pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
+                            w.w = pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+                        }
+                        *reinterpret_cast<uint4*>(out + c * 16 + i * 8) = w;
+                    }
+                }
+                tc_fence_before();
+            }
+            // rows key by key, by the whole warp
             for (uint32_t rows = __ballot_sync(0xffffffffu, odd); rows; rows &= rows - 1) {
                 const uint32_t r = quarter * 32 + __ffs(rows) - 1, token = p.per.div(r);
                 paged_row<bf16>(p, it.s, it.seq, it.seq.start + it.token0 + t * prm.tokens + token, it.kvh * p.per.d + r - token * p.per.d, lane);
             }
         }
     }
-
     teardown();
 }
 
@@ -597,24 +815,29 @@ static bool pp_map(CUtensorMap* map, const void* base, uint32_t rank, const uint
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+uint64_t paged_prompt_workspace_bytes(uint32_t dim, uint32_t vdim) {
+    const uint32_t w = std::max(dim, vdim) <= 64 ? 64 : 128;
+    return std::max(dim, vdim) > 128 ? 0 : PAGED_COUNTERS + (uint64_t)PP_BLOCKS * 2 * 2 * 128 * (w + 2) * 4;
+}
+
 bool paged_prompt_eligible(const PagedAttention& a, int dtype) {
     const uint64_t strides = (uint64_t)a.dim | a.vdim | a.k_page | a.k_row | a.k_head | a.v_page | a.v_row | a.v_head | a.q_ld | a.out_ld | a.page_rows;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
     const uint64_t most = std::max({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head});
     const uint64_t least = std::min({a.k_page, a.k_row, a.k_head, a.v_page, a.v_row, a.v_head});
     return dtype == TNSR_B200_BF16 && a.dim <= 128 && a.vdim <= 128 && strides % 8 == 0 && at % 16 == 0 && a.scale > 0.0f && a.heads / a.kv_heads <= 128 &&
-           least > 0 && most < (1ull << 38) && a.pool_pages < 0x7fffffffu && g_gemm_engine != 1 && encode_fn() != nullptr;
+           (uint64_t)a.sequences * a.kv_heads * ceil_div(a.chunk, 2 * (128 / (a.heads / a.kv_heads))) < 0x7fffff00u && least > 0 && most < (1ull << 38) && a.pool_pages < 0x7fffffffu && g_gemm_engine != 1 && encode_fn() != nullptr;
 }
 
-template <int W>
+template <int W, bool DIVIDED>
 static int launch_prompt_width(const PromptParams& prm, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
-    if (const int rc = allow_shared<paged_prompt_kernel<W>>(PromptShape<W>::BYTES, "paged_attention attribute")) return rc;
+    constexpr uint32_t bytes = PromptShape<W>::BYTES + (DIVIDED ? sizeof(PromptPlan) : 0);
+    if (const int rc = allow_shared<paged_prompt_kernel<W, DIVIDED>>(bytes, "paged_attention attribute")) return rc;
     int dev = 0, sms = 0;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const uint64_t items = (uint64_t)prm.p.a.sequences * prm.p.a.kv_heads * prm.pairs;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(items, sms > 0 ? sms : 148);
-    launch_kernel(paged_prompt_kernel<W>, dim3(grid), dim3(PP_THREADS), (size_t)PromptShape<W>::BYTES, stream, mq, mk, mv, prm);
+    const uint32_t most = std::min<uint32_t>(sms > 0 ? sms : PP_BLOCKS, PP_BLOCKS), grid = DIVIDED ? most : std::min(prm.items, most);
+    launch_kernel(paged_prompt_kernel<W, DIVIDED>, dim3(grid), dim3(PP_THREADS), (size_t)bytes, stream, mq, mk, mv, prm);
     return TNSR_B200_OK;
 }
 
@@ -624,8 +847,20 @@ int launch_paged_prompt(const PagedParams& p, cudaStream_t stream) {
     prm.p = p;
     prm.tokens = 128 / p.per.d;
     prm.pairs = ceil_div(a.chunk, 2 * prm.tokens);
+    prm.units = a.sequences * a.kv_heads;
+    prm.items = prm.units * prm.pairs;           // fewer than 2^31: paged_prompt_eligible
     prm.box = std::min(128u, a.page_rows & (0u - a.page_rows));
     prm.wait_limit_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+    // The last round is divided where it can pay: items of more key blocks than the joins cost, and (as far as can be told here) a round that leaves a quarter of
+    // the grid idle.  One prompt of 6000 rows over 12000 keys, window 4096, 32 / 8 heads: 487 -> 460 us; 3 x 100 rows over up to 4000 keys: 74 -> 47; where nothing
+    // pays the plan alone costs 2 to 4 us.
+    const uint64_t entries = (uint64_t)a.sequences * prm.pairs;
+    const uint32_t span = a.window ? (uint32_t)std::min<uint64_t>(p.capacity, (uint64_t)a.window + 2 * prm.tokens + std::min(a.sinks, p.capacity) + 256) : p.capacity;
+    const uint32_t most = ceil_div(span, 128u), left = prm.items % PP_BLOCKS;
+    const bool divided = a.workspace && entries <= PP_ENTRIES && most - most / PP_PARTS > PP_JOIN &&
+                         (a.row_starts || (left > 0 && left < PP_BLOCKS * 3 / 4));
+    prm.done = divided ? reinterpret_cast<uint32_t*>(a.workspace) : nullptr;
+    prm.partial = divided ? reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.workspace) + PAGED_COUNTERS) : nullptr;
     CUtensorMap mq, mk, mv;
     const uint64_t q_dims[3] = {a.dim, a.heads, a.rows}, q_strides[2] = {a.dim, a.q_ld};
     const uint32_t q_box[3] = {64, p.per.d, prm.tokens}, kv_box[4] = {64, 1, prm.box, 1};
@@ -636,7 +871,9 @@ int launch_paged_prompt(const PagedParams& p, cudaStream_t stream) {
         set_thread_error("paged_attention: tensor map encoding failed");
         return TNSR_B200_ERR_CUDA;
     }
-    return std::max(a.dim, a.vdim) <= 64 ? launch_prompt_width<64>(prm, mq, mk, mv, stream) : launch_prompt_width<128>(prm, mq, mk, mv, stream);
+    if (std::max(a.dim, a.vdim) <= 64)
+        return divided ? launch_prompt_width<64, true>(prm, mq, mk, mv, stream) : launch_prompt_width<64, false>(prm, mq, mk, mv, stream);
+    return divided ? launch_prompt_width<128, true>(prm, mq, mk, mv, stream) : launch_prompt_width<128, false>(prm, mq, mk, mv, stream);
 }
 
 }  // namespace tb

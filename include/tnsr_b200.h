@@ -795,8 +795,11 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
 
 /* The `keep` best of a group's beams x vocabulary candidates, best first.
  *     score(b, t) = scores[b] + (logits[b, t] - log sum_j exp logits[b, j])
- * in f64.  Of equal scores the earlier beam comes first, of a beam's equal logits
- * the smaller token.  A finished beam has one candidate, end_token with scores[b]
+ * in f64, the row's largest logit taken off before the sum's logarithm, so that
+ * finite logits of any size count as they are (tokens masked by the type's lowest
+ * value as well as by -inf; a row of nothing but one such value is a uniform one).
+ * Of equal scores the earlier beam comes first, then the larger logit, then the
+ * smaller token.  A finished beam has one candidate, end_token with scores[b]
  * as it is; its other tokens count as -inf, and so do all tokens of a beam whose
  * score is not finite or whose logits hold NaN, +inf or nothing but -inf (such
  * tokens fill up what better ones leave, by beam and token).  logits

@@ -6,13 +6,13 @@
 // A finished beam has one candidate with its own score, the end token; its other tokens, and all of a beam whose sum or score is no finite
 // number (a NaN or +inf logit, nothing but -inf, a score of -inf), count as -inf.
 //
-// beam_scan_kernel reads every logit once: a block has a run of a row, a thread's values pass through its registers, 32 at a time, and leave their maximum and their
+// beam_scan_kernel reads every logit once: a block has a run of a row, a thread's values pass through its registers, 16 at a time, and leave their maximum and their
 // sum of exponentials.  The largest of the warps' threads bound the keep-th best value from below; threads that have one at or above the bound have
 // their values read again, and what is at or above it is gathered and ranked by counting: keep and a few more.  Keys are (value, index) pairs, so no
 // two are equal.  Where equal values (masked tokens, say) let too many in, the run is gone through once more by keys alone.  The block that comes last
 // of a group's joins its runs in the same way.
 //
-// Sums: 32 terms in f32, the rest in f64.  A block's order of terms does not depend on the row, so that equal rows have equal sums to the last bit.
+// Sums: 16 terms in f32, the rest in f64.  A block's order of terms does not depend on the row, so that equal rows have equal sums to the last bit.
 // Bound by HBM (each logit once) for large groups, else by the chain of barriers behind the reading: 48 groups x 6 beams x 50021 logits, keep 12, 22.6 us =
 // 2.55 TB/s (one wave of blocks: reading is half of it); one group x 4 beams x 32000, keep 4, 9.8 us.
 #include <algorithm>
@@ -44,11 +44,14 @@ __device__ __forceinline__ float bs_ex2(float x) {
     return y;
 }
 
-// sum_j exp x_j of a run is sum * exp(base); base is about the largest x.
+// sum_j exp x_j of a run is sum * exp(base); base is the largest x.
 struct BeamRun {
     double sum, base;
 };
 constexpr float BS_LOG2E = 1.4426950408889634f;
+// exp(x - base) for x <= base, or NaN for a base of +inf: the difference first, so that logits of any finite size have terms of at most 1 (a base times log2(e) would
+// overflow, or be rounded by more than an exponent holds, for the large negative numbers that mask tokens).
+__device__ __forceinline__ float bs_term(float x, float base) { return bs_ex2((x - base) * BS_LOG2E); }
 
 // ---- a group's runs joined ----------------------------------------------------------------------------------------------------
 // Larger is better: score, then beam, logit and token in one word.
@@ -85,7 +88,7 @@ static uint32_t merge_room(const MergeShape& m, uint32_t keep) { return m.bounds
 // By one block.  `space`: [lists] at the place of the bound, what is gathered, and (`staged`) the lists.
 __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, const MergeShape& shape, uint32_t room, bool staged, const BeamRun* parts,
                            const uint64_t* lists, BeamCandidate* space) {
-    __shared__ double offset[BEAM_MAX];           // of a beam's logits; NaN: all of its candidates are -inf
+    __shared__ double base_of[BEAM_MAX], log_sum[BEAM_MAX], score_of[BEAM_MAX];     // a beam's largest logit, log sum exp(x - largest) (NaN: all of its candidates are -inf), score
     __shared__ uint8_t ended[BEAM_MAX], was[BEAM_MAX];
     __shared__ BeamCandidate bound;
     __shared__ uint32_t places[BS_WARPS];
@@ -112,8 +115,10 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
         if (lane == 0) {
             was[beam] = over;
             ended[beam] = over && b.end_token < b.vocab && isfinite(c);
-            const double total = top + log(sum);
-            offset[beam] = !over && isfinite(total) && isfinite(c) ? (double)c - total : nan("");
+            const double total = log(sum);
+            base_of[beam] = top;
+            log_sum[beam] = !over && isfinite(top) && isfinite(total) && isfinite(c) ? total : nan("");
+            score_of[beam] = c;
         }
     }
     if (tid == 0) count = 0;
@@ -121,8 +126,7 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
     // entry `i` of list `l` (run l % runs of beam l / runs); a beam without sums has one list that counts
     auto entry = [&](uint32_t l, uint32_t i) -> BeamCandidate {
         const uint32_t beam = l / runs;
-        const double o = offset[beam];
-        if (isnan(o)) {
+        if (isnan(log_sum[beam])) {
             if (l % runs) return {0, 0};
             uint32_t token = i;
             if (ended[beam]) {
@@ -133,7 +137,8 @@ __device__ void beam_merge(const BeamSelect& b, uint32_t group, uint32_t runs, c
         }
         const uint64_t key = staged ? copy[l * b.keep + i] : __ldcg(entries + (uint64_t)l * b.keep + i);
         if (key == 0) return {0, 0};
-        return bs_candidate(o + bs_value((uint32_t)(key >> 32)), beam, (uint32_t)(key >> 32), ~(uint32_t)key);
+        // the largest logit goes first: beside one of 10^20 the sum's logarithm would be lost
+        return bs_candidate(score_of[beam] + (((double)bs_value((uint32_t)(key >> 32)) - base_of[beam]) - log_sum[beam]), beam, (uint32_t)(key >> 32), ~(uint32_t)key);
     };
     // The bound.  If the q-th largest of the lists' entries at place p has (p + 1) q >= keep, so many entries are at or above it.  Few lists: by scores rounded
     // down to f32, a warp each for places 0, 1, 3, 7, ..., and the largest of what they find (heads alone let all of a good beam's lists in where the beams
@@ -359,9 +364,8 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
     if (tid == 0)
         for (uint32_t i = 0; i < min(pieces, BS_STAGES); ++i) fetch(i);
 
-    // The thread's largest value and its sum of exponentials.  A term is 2^(x L + shift) with L the float nearest to log2(e): the base of the sum is what the
-    // rounded shift stands for and not the maximum it was made from, or all terms would be off by the same factor.
-    float mine = -INFINITY, shift = 0.0f;
+    // The thread's largest value and its sum of exponentials of what the others are below it.
+    float mine = -INFINITY;
     double sum = 0.0;
     for (uint32_t i = 0; i < pieces; ++i) {
         const uint32_t stage = i % BS_STAGES, base = first + i * BS_PIECE, here = min(end - base, BS_PIECE);
@@ -407,14 +411,13 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
 #pragma unroll
         for (int j = 1; j < 16; ++j) largest = fmaxf(largest, v[j]);
         if (largest > mine) {
-            const float now = -largest * BS_LOG2E;
-            if (mine != -INFINITY) sum *= bs_ex2(now - shift);
+            if (mine != -INFINITY) sum *= bs_term(mine, largest);
             mine = largest;
-            shift = now;
         }
+        const float base_value = mine == -INFINITY ? 0.0f : mine;       // -inf alone: terms of 0
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[j & 3] += bs_ex2(fmaf(v[j], BS_LOG2E, shift));
+        for (int j = 0; j < 16; ++j) part[j & 3] += bs_term(v[j], base_value);
         sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
     }
     if (gave_up) {                       // copies that are still on their way get time to land
@@ -456,8 +459,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
     // is done exactly.
     if (mine >= low && low != -INFINITY) listed[atomicAdd(&threads, 1u)] = (uint8_t)tid;
     // the sums at one base
-    const float block_shift = top == -INFINITY ? 0.0f : -top * BS_LOG2E;
-    if (mine != -INFINITY) sum *= bs_ex2(block_shift - shift);      // what had no finite number has a sum of 0, or of NaN
+    if (mine != -INFINITY) sum *= bs_term(mine, top);               // what had no finite number has a sum of 0, or of NaN
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) sums[warp] = sum;
@@ -494,8 +496,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
     double total = 0.0;
 #pragma unroll
     for (int w = 0; w < (int)BS_WARPS; ++w) total += sums[w];
-    const double old_base = top == -INFINITY ? -INFINITY : -(double)block_shift / BS_LOG2E;
-    if (tid == 0) runs[blockIdx.x] = {total, old_base};
+    if (tid == 0) runs[blockIdx.x] = {total, (double)top};
     if (tid < keep) lists[(uint64_t)blockIdx.x * keep + tid] = tid < kept ? best[tid] : 0;
     if (!tickets) return;
     // the block that comes last joins the group's runs

@@ -788,8 +788,9 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
  *    pools and rows is read or written in such a case.
  *  - A workspace is device memory, 16-byte aligned, zeroed once before its first
  *    use (again if a launch was cut short by a device error); calls leave it ready
- *    for the next one.  Calls that may overlap on the GPU must not share one, and
- *    two captured graphs that share one must not run at the same time.
+ *    for the next one, of the same operator at any sizes that it is large enough for.
+ *    Calls that may overlap on the GPU must not share one, and two captured graphs
+ *    that share one must not run at the same time.
  *  - Descriptions are read before a call returns; host arrays of pointers and sizes
  *    too. */
 
@@ -820,6 +821,7 @@ typedef struct tnsr_b200_beam_select_args {
     uint32_t groups, beams, vocab, keep, end_token;
     int32_t dtype;
 } tnsr_b200_beam_select_args;
+/* Enough for calls of fewer groups, beams, tokens and candidates too. */
 TNSR_B200_API uint64_t tnsr_b200_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep);
 TNSR_B200_API int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, void* stream);
 

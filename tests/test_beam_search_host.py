@@ -131,3 +131,13 @@ def test_rows_over_pages_refuse(library, make, entry):
         need = library.tnsr_b200_paged_attention_workspace(64, 64, 1)
         refuses(call(C.byref(make(workspace_bytes=need - 1)), None), "workspace")
         refuses(call(C.byref(make(workspace=SOME + 8)), None), "workspace")
+
+
+def test_a_selections_workspace_is_enough_for_smaller_ones(library):
+    need = library.tnsr_b200_beam_select_workspace
+    for vocab in (5, 2049, 9000, 130001):
+        for beams in (1, 4, 7, 32):
+            sizes = [need(groups, beams, vocab, 8) for groups in range(1, 200)]
+            assert sizes == sorted(sizes)
+    for big, small in (((40, 8, 50000, 16), (39, 3, 50000, 16)), ((40, 8, 50000, 16), (40, 8, 2048, 16)), ((40, 8, 50000, 16), (1, 1, 49999, 1))):
+        assert need(*big) >= need(*small)

@@ -18,6 +18,8 @@ struct BeamSelect {
 };
 constexpr uint32_t BEAM_MAX = 32, BEAM_MAX_KEEP = 64;
 constexpr uint32_t BEAM_MAX_VOCAB = 1u << 26;
+// Bytes of a workspace before the lists: the groups' tickets, zero between calls.  A fixed place, so that a call of other sizes finds no other call's lists there.
+constexpr uint32_t BEAM_COUNTERS = 4096;
 uint64_t beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep);
 int launch_beam_select(const BeamSelect& b, int dtype, cudaStream_t stream);
 

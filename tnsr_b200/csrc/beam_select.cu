@@ -529,8 +529,9 @@ static BeamPlan beam_plan(uint64_t rows, uint32_t vocab) {
 }
 
 uint64_t beam_select_workspace_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep) {
-    const uint64_t rows = (uint64_t)groups * beams;
-    return rows * beam_plan(rows, std::max(vocab, 1u)).runs * (sizeof(BeamRun) + 8ull * keep) + 4ull * groups;
+    // rows x runs of beam_plan at the most, for this call and for all with no more groups, beams, vocabulary and candidates: fewer rows have more runs each
+    const uint64_t rows = (uint64_t)groups * beams, most = std::min<uint64_t>(BS_RUNS, ceil_div(std::max(vocab, 1u), BS_LEAST_RUN));
+    return BEAM_COUNTERS + std::max(rows, std::min<uint64_t>(BS_BLOCKS, rows * most)) * (sizeof(BeamRun) + 8ull * keep);
 }
 
 template <typename T>
@@ -545,13 +546,14 @@ static int launch_scan(const BeamSelect& b, const BeamPlan& p, BeamRun* runs, ui
 int launch_beam_select(const BeamSelect& b, int dtype, cudaStream_t stream) {
     if (b.groups == 0) return TNSR_B200_OK;
     const BeamPlan p = beam_plan((uint64_t)b.groups * b.beams, b.vocab);
-    uint64_t* lists = reinterpret_cast<uint64_t*>(b.workspace);
+    uint32_t* tickets = reinterpret_cast<uint32_t*>(b.workspace);
+    uint64_t* lists = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(b.workspace) + BEAM_COUNTERS);
     BeamRun* runs = reinterpret_cast<BeamRun*>(lists + (uint64_t)b.groups * b.beams * p.runs * b.keep);
-    uint32_t* tickets = reinterpret_cast<uint32_t*>(runs + (uint64_t)b.groups * b.beams * p.runs);
     const MergeShape shape = merge_shape(b.beams, p.runs, b.keep);
     const uint32_t room = merge_room(shape, b.keep), bytes = (uint32_t)sizeof(BeamCandidate) * (shape.lists + room), list_bytes = shape.lists * b.keep * 8;
-    // joined by a group's last block where that has the shared memory for it, else by a launch of its own
-    const bool joined = bytes + list_bytes <= BS_GATHER * 8, staged = joined || list_bytes <= BS_STAGED;
+    // joined by a group's last block where that has the shared memory for it and the group a ticket, else by a launch of its own (2 us of the 40 or more that over a
+    // thousand groups take)
+    const bool joined = bytes + list_bytes <= BS_GATHER * 8 && b.groups <= BEAM_COUNTERS / 4, staged = joined || list_bytes <= BS_STAGED;
     int rc = dtype == TNSR_B200_F32 ? launch_scan<float>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream)
                                     : launch_scan<bf16>(b, p, runs, lists, shape, room, staged, joined ? tickets : nullptr, stream);
     if (rc) return rc;

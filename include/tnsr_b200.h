@@ -788,7 +788,8 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
  *    pools and rows is read or written in such a case.
  *  - A workspace is device memory, 16-byte aligned, zeroed once before its first
  *    use (again if a launch was cut short by a device error); calls leave it ready
- *    for the next one, of the same operator at any sizes that it is large enough for.
+ *    for the next one, of the same operator (fork, reserve and compact: of any of
+ *    them, on any book) at any sizes that it is large enough for.
  *    Calls that may overlap on the GPU must not share one, and two captured graphs
  *    that share one must not run at the same time.
  *  - Descriptions are read before a call returns; host arrays of pointers and sizes

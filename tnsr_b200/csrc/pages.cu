@@ -25,7 +25,7 @@ namespace tb {
 constexpr uint32_t PG_NONE = 0xffffffffu;
 constexpr uint32_t PG_THREADS = 1024;
 
-// Workspace in u32: [0] pairs to copy, [1] ticket of fork; then lists.  Zero between calls: ticket, keeper, writers.
+// Workspace in u32: [0] pairs to copy, [1] ticket of fork, zero between calls; then lists that every call fills for itself, for their places follow the book's sizes.
 struct PageScratch {
     uint32_t *header, *keeper, *writers, *pages, *from, *to, *need, *copy, *source;
 };
@@ -299,6 +299,12 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
         }
         if (b.holders[page] < 2) continue;
         ws.source[s] = page;
+        ws.writers[page] = ws.keeper[page] = 0;
+    }
+    __syncthreads();
+    for (uint32_t s = s0; s < s1; ++s) {
+        const uint32_t page = ws.source[s];
+        if (page == PG_NONE) continue;
         atomicAdd(ws.writers + page, 1u);
         atomicMax(ws.keeper + page, ~s);
     }
@@ -318,13 +324,6 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
     }
     uint32_t all, all_copies;
     uint32_t at = block_scan(want, all), copy_at = block_scan(copies, all_copies);
-    // zero between calls: whoever raised them
-    for (uint32_t s = s0; s < s1; ++s) {
-        const uint32_t length = b.lengths[s], n = rows ? rows[s] : rows_each;
-        if ((uint64_t)length + n > room || n == 0 || length % b.page_rows == 0) continue;
-        const uint32_t page = *last_entry(s, length);
-        if (page < b.pool_pages) ws.writers[page] = ws.keeper[page] = 0;
-    }
     if (bad) {
         if (threadIdx.x == 0) report(b.d_status, bad);
         return;

@@ -9,6 +9,7 @@
 //                 of any strides; a box is the largest power of two of rows that divides a page, lane i of the warp looks box i's page up and asks for
 //                 it.  Boxes that are not wanted, or whose page lies outside the pool, get coordinates outside: zeros.
 //   warp 1        one thread issues S = Q K^T (128 x 128) and O += P V (128 x W), per tile: P V of block j, then S of block j + 1.
+//   warp 2        looks through the values of blocks that are seen in part, before any product has them (below).
 //   warps 4-7, 8-11   softmax of tile 0 and 1, a thread per row: no exchange between threads.  The row's weights go back over its
 //                 scores as bf16 (the A operand in TMEM).  O stays in TMEM through an item and is rescaled only when a row's maximum has
 //                 grown by more than 2^8 since the last time (weights then are at most 2^8, sums f32); S of block j is complete only when
@@ -21,7 +22,8 @@
 //
 // Values that some rows of an item see and others do not may hold infinities or NaN, which a weight of 0 does not keep out, and so may the
 // rest of a last page: in blocks that are not seen by all, each row of values is looked through and such elements are zeroed before the
-// product; rows that see one of them are computed once more key by key.
+// product; rows that see one of them are computed once more key by key.  One warp does that for both tiles: it alone changes values, each block passes it on its way to
+// the products, and its list of an item's keys is read when the item is complete.  It takes the time in which the block's scores become weights.
 //
 // Every wait is bounded as elsewhere: one that gives up raises the abort flag, the roles fall through and the status word is set.
 //
@@ -36,7 +38,7 @@
 namespace tb {
 
 constexpr uint32_t PP_THREADS = 384;
-constexpr uint32_t PP_ODD = 16;                      // keys with values of no finite number that a tile remembers
+constexpr uint32_t PP_ODD = 16;                      // keys with values of no finite number that an item's list holds
 constexpr uint32_t PP_HALF = 128 * 128;              // 128 rows of 64 bf16
 
 template <int W>
@@ -331,12 +333,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     uint8_t* v_ring = k_ring + STAGES * S::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(v_ring + STAGES * S::TILE);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8;       // a tile each
-    uint64_t *looked = bars + 10;                              // a tile each: its warps are through with an item's values
-    uint64_t *k_full = bars + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + STAGES);
+    uint64_t *met = bars + 10;                                 // a tile each: its warps wait for one another when they join
+    uint64_t *listed = bars + 12, *read = bars + 14;           // items of even and odd number: their list is complete; all have read it
+    uint64_t *k_full = bars + 16, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES, *v_clean = v_empty + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + STAGES);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* odd_seen = tmem_slot + 2;                        // [2 tiles][2]: last item of even or odd number in which something was found, and how many keys
-    uint32_t* odd_keys = odd_seen + 4;                         // [2 tiles][2][PP_ODD]
+    uint32_t* odd_count = tmem_slot + 2;                       // [2]: of the lists
+    uint32_t* odd_keys = odd_count + 2;                        // [2][PP_ODD]
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedParams& p = prm.p;
     const uint64_t limit = prm.wait_limit_ns;
@@ -348,14 +351,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             mbar_init(s_full + t, 1);
             mbar_init(p_full + t, 4);
             mbar_init(o_full + t, 1);
-            mbar_init(looked + t, 4);
-            odd_seen[2 * t] = odd_seen[2 * t + 1] = 0;
+            mbar_init(met + t, 4);
+            mbar_init(listed + t, 1);
+            mbar_init(read + t, 8);
         }
         for (uint32_t i = 0; i < STAGES; ++i) {
             mbar_init(k_full + i, 1);
             mbar_init(k_empty + i, 1);
             mbar_init(v_full + i, 1);
             mbar_init(v_empty + i, 1);
+            mbar_init(v_clean + i, 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -507,7 +512,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         then[1] = tile_sees(p, it, 1, key0);
                         ok = mbar_wait(k_full + next, next_parity, abort_flag, limit);
                     }
-                    ok = ok && mbar_wait(v_full + stage, parity, abort_flag, limit);
+                    ok = ok && mbar_wait(v_full + stage, parity, abort_flag, limit) && mbar_wait(v_clean + stage, parity, abort_flag, limit);
                     if (!ok) break;
                     const uint32_t v = v_low + stage * (S::TILE >> 4);
 #pragma unroll
@@ -537,6 +542,60 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 blocks += j1 - j0;
             }
         }
+    } else if (warp == 2) {
+        // ---------------- values of no finite number ----------------
+        uint32_t blocks = 0, number = 0;             // key blocks; items so far
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
+        bool ok = true;
+        while (ok && walk.more(prm, plan)) {
+            if (!walk.step(prm, plan, it) || it.blocks == 0) continue;
+            const uint32_t j0 = walk.begin(), j1 = walk.end(it), slot = number & 1;
+            // the list was that of the item before the last one
+            if (number >= 2 && !wait(read + slot, ((number >> 1) - 1) & 1)) break;
+            uint32_t count = 0;
+            for (uint32_t j = j0; j < j1; ++j, ++blocks) {
+                const uint32_t stage = blocks % STAGES, key0 = item_key0(it, j);
+                ok = wait(v_full + stage, (blocks / STAGES) & 1);
+                if (!ok) break;
+                if (partly_seen(p, it, 0, it.tokens[1] ? 1 : 0, key0)) {
+                    // a row a lane, four times
+                    for (uint32_t row = lane; row < 128; row += 32) {
+                        uint8_t* v_row = v_ring + stage * S::TILE + row * 128;
+                        // the order of the pieces by lane: neighbours read other banks.  An exponent of ones carries into the sign's place.
+                        uint32_t ones = 0;
+#pragma unroll
+                        for (uint32_t i = 0; i < 8 * HALVES; ++i) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(v_row + (i / 8) * PP_HALF + ((i + lane) & 7) * 16);
+                            ones |= ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
+                                    ((x.w & 0x7f807f80u) + 0x00800080u);
+                        }
+                        const bool found = ones & 0x80008000u;
+                        if (found) {
+#pragma unroll 1
+                            for (uint32_t i = 0; i < 32 * HALVES; ++i) {
+                                uint32_t* x = reinterpret_cast<uint32_t*>(v_row + (i / 32) * PP_HALF) + i % 32;
+                                const uint32_t v = *x, odd = ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                                if (odd) *x = v & ~((odd & 0x8000u ? 0xffffu : 0u) | (odd & 0x80000000u ? 0xffff0000u : 0u));
+                            }
+                        }
+                        __syncwarp();
+                        const uint32_t key = key0 + row;
+                        const bool note = found && (int32_t)key <= it.high && ((int32_t)key >= it.from[0] || key < p.a.sinks);
+                        const uint32_t notes = __ballot_sync(0xffffffffu, note), place = count + __popc(notes & ((1u << lane) - 1));
+                        if (note && place < PP_ODD) odd_keys[slot * PP_ODD + place] = key;
+                        count += __popc(notes);
+                    }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_clean + stage);
+            }
+            if (!ok) break;
+            if (lane == 0) odd_count[slot] = count;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(listed + slot);
+            ++number;
+        }
     }
     teardown();
     return;
@@ -548,64 +607,44 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t s_addr = tmem + t * 128 + ((quarter * 32u) << 16), o_addr = tmem + PP_O + t * W + ((quarter * 32u) << 16);
         const uint32_t my_token = p.per.div(row), my_head = row - my_token * p.per.d;
-        uint32_t blocks = 0, seen = 0, outputs = 0, number = 0, looks = 0;      // key blocks; blocks of the tile; outputs; items; turns of `looked` so far
+        uint32_t seen = 0, outputs = 0, number = 0, meets = 0;      // blocks of the tile; its outputs; items with keys; turns of `met` so far
         bool ok = true;
         // a warp gives up as a whole
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
         while (ok && walk.more(prm, plan)) {
             if (!walk.step(prm, plan, it)) continue;
             const uint32_t j0 = walk.begin(), j1 = walk.end(it);
+            // the item's list, once it is complete: which keys' values must not be multiplied by 0 (`mine`, the row sees one of them).  Every warp takes every list.
+            auto odd_in_sight = [&](bool mine, int32_t at) {
+                const uint32_t slot = number & 1;
+                if (!wait(listed + slot, (number >> 1) & 1)) ok = false;
+                const uint32_t count = *(volatile uint32_t*)(odd_count + slot);
+                bool odd = count > PP_ODD;
+                if (mine)
+                    for (uint32_t i = 0; i < min(count, PP_ODD); ++i) {
+                        const uint32_t key = *(volatile uint32_t*)(odd_keys + slot * PP_ODD + i);
+                        odd |= (int32_t)key <= at && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > at);
+                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(read + slot);
+                ++number;
+                return odd && mine;
+            };
             if (!it.tokens[t]) {
-                blocks += j1 - j0;
+                if (it.blocks) odd_in_sight(false, 0);
                 continue;
             }
             const int32_t at = it.first[t] + (int32_t)min(my_token, it.tokens[t] - 1);
-            ++number;
             const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
             float m = -INFINITY, l = 0.0f;
             bool any = false;
             for (uint32_t j = j0; j < j1; ++j) {
-                const uint32_t b = blocks + (j - j0), key0 = item_key0(it, j);
+                const uint32_t key0 = item_key0(it, j);
                 if (!tile_sees(p, it, t, key0)) continue;
                 any = true;
                 if (!wait(s_full + t, seen & 1)) { ok = false; break; }
                 ++seen;
                 tc_fence_after();
-                if (partly_seen(p, it, 0, it.tokens[1] ? 1 : 0, key0)) {
-                    // a row of values per thread.  Behind s_full: the products' thread has by then waited for the values of every earlier block, so that
-                    // the ring cannot be a whole turn behind, which a barrier's parity would not show
-                    if (!wait(v_full + b % STAGES, (b / STAGES) & 1)) { ok = false; break; }
-                    uint8_t* v_row = v_ring + (b % STAGES) * S::TILE + row * 128;
-                    // the order of the pieces by lane: neighbours read other banks.  An exponent of ones carries into the sign's place.
-                    uint32_t ones = 0;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8 * HALVES; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(v_row + (i / 8) * PP_HALF + ((i + lane) & 7) * 16);
-                        ones |= ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
-                                ((x.w & 0x7f807f80u) + 0x00800080u);
-                    }
-                    const bool found = ones & 0x80008000u;
-                    if (found) {
-#pragma unroll 1
-                        for (uint32_t i = 0; i < 32 * HALVES; ++i) {
-                            uint32_t* x = reinterpret_cast<uint32_t*>(v_row + (i / 32) * PP_HALF) + i % 32;
-                            const uint32_t v = *x, odd = ((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                            if (odd) *x = v & ~((odd & 0x8000u ? 0xffffu : 0u) | (odd & 0x80000000u ? 0xffff0000u : 0u));
-                        }
-                    }
-                    const uint32_t key = key0 + row;
-                    if (found && (int32_t)key <= it.high && ((int32_t)key >= it.from[0] || key < p.a.sinks)) {
-                        const uint32_t slot = 2 * t + (number & 1);
-                        uint32_t now = *(volatile uint32_t*)(odd_seen + slot), then;
-                        do {
-                            then = now;
-                            now = atomicCAS(odd_seen + slot, then, then >> 8 != number ? number << 8 | 1u : min(then + 1, number << 8 | 255u));
-                        } while (now != then);
-                        const uint32_t place = then >> 8 != number ? 0u : then & 255u;
-                        if (place < PP_ODD) odd_keys[slot * PP_ODD + place] = key;
-                    }
-                    fence_proxy_async_smem();
-                }
                 __syncwarp();
                 float v[128];
 #pragma unroll
@@ -678,28 +717,15 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + t);
             }
-            blocks += j1 - j0;
             if (!ok) break;
             if (any) {
                 if (!wait(o_full + t, outputs & 1)) { ok = false; break; }
                 ++outputs;
                 tc_fence_after();
             }
-            // whether the row sees something that must not be multiplied by 0 (a warp that is ahead writes to the other place)
-            __syncwarp();
-            if (lane == 0) mbar_arrive(looked + t);
-            if (!wait(looked + t, (DIVIDED ? looks++ : number - 1) & 1)) { ok = false; break; }
-            bool mine = my_token < it.tokens[t], odd = false;
-            const uint32_t slot = 2 * t + (number & 1), found = *(volatile uint32_t*)(odd_seen + slot);
-            if (found >> 8 == number) {
-                odd = (found & 255u) > PP_ODD;
-                for (uint32_t i = 0; i < min(found & 255u, PP_ODD); ++i) {
-                    const uint32_t key = odd_keys[slot * PP_ODD + i];
-                    odd |= (int32_t)key <= at && (!p.a.window || key < p.a.sinks || (int64_t)key + p.a.window > at);
-                }
-                odd &= mine;
-                mine &= !odd;
-            }
+            bool mine = my_token < it.tokens[t], odd = it.blocks && odd_in_sight(mine, at);
+            if (!ok) break;
+            mine &= !odd;
             bf16* out = reinterpret_cast<bf16*>(p.a.out) + (uint64_t)(it.seq.start + it.token0 + t * prm.tokens + my_token) * p.a.out_ld +
                         (uint64_t)(it.kvh * p.per.d + my_head) * p.a.vdim;
             bool joined = false;                     // or left to be
@@ -720,8 +746,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     dst[(W + 1) * 128] = l;
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(looked + t);
-                    if (!wait(looked + t, looks++ & 1)) { ok = false; break; }
+                    if (lane == 0) mbar_arrive(met + t);
+                    if (!wait(met + t, meets++ & 1)) { ok = false; break; }
                     const uint32_t item_at = plan.before[walk.number - 1 - plan.divided], c0 = item_at / plan.length,
                                    parts = (item_at + it.blocks - 1) / plan.length - c0 + 1;
                     if (row == 0) {
@@ -732,8 +758,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         join_now[t] = last;
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(looked + t);
-                    if (!wait(looked + t, looks++ & 1)) { ok = false; break; }
+                    if (lane == 0) mbar_arrive(met + t);
+                    if (!wait(met + t, meets++ & 1)) { ok = false; break; }
                     if (!join_now[t]) continue;
                     const bool there = my_token < it.tokens[t];
                     const float* tile = prm.partial + ((uint64_t)c0 * 4 + t) * 128 * (W + 2) + row;

@@ -777,7 +777,8 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
  *     pages_fork       sequences take over their parents' pages (reorder_states:
  *                      recurrent states, contiguous caches)
  *     pages_reserve    room for the next row; pages that others hold too are copied
- *     per layer: paged_append (new keys and values), paged_attention
+ *     per layer: paged_append (new keys and values; not where the reserve was
+ *                refused), paged_attention
  * All of it is device work on the caller's stream, without synchronisation.  The
  * entry points below share these rules.
  *  - A status word (`d_status`, a device int that the caller clears, may be NULL)
@@ -845,6 +846,7 @@ typedef struct tnsr_b200_page_book {
     int* d_status;
     uint64_t workspace_bytes;
     uint32_t sequences, table_ld, page_rows, pool_pages;
+    uint32_t* refused;            /* device word or NULL: every reserve writes 0, or why it was refused (3, 4, 5) */
 } tnsr_b200_page_book;
 /* The pools that a book speaks of (keys and values of every layer): page i of pool t
  * is page_bytes[t] bytes at tensors[t] + i * page_bytes[t].  `tensors` and
@@ -864,7 +866,10 @@ TNSR_B200_API int tnsr_b200_pages_fork(const tnsr_b200_page_book* book, const ui
  * hold too is replaced by a copy in all pools, for every sequence that gets rows
  * but the first one of them if nobody else holds the page.  If the free pages do
  * not suffice (5), or a sequence would outgrow its table row (3), or a last page's
- * entry is not one (4), the status word says so and nothing has changed. */
+ * entry is not one (4), the status word and book->refused say so and nothing has
+ * changed: the lengths are the old ones, so that rows appended now would be written
+ * over the newest old ones, in pages that others may hold.  A step that is queued or
+ * captured without looking at the status in between gives paged_append `refused`. */
 TNSR_B200_API int tnsr_b200_pages_reserve(const tnsr_b200_page_book* book, const tnsr_b200_page_pools* pools, const uint32_t* rows,
                                           uint32_t rows_each, void* stream);
 /* Sequences s with gone[s] != 0 (device bytes) give their pages back and have length 0. */
@@ -887,7 +892,8 @@ TNSR_B200_API int tnsr_b200_pages_copy(const tnsr_b200_page_pools* pools, const 
  * vdim: slices of a fused projection will do.  Element (page, row, head, i) of a
  * pool lies at page * k_page + row * k_row + head * k_head + i, in elements; three
  * zeros stand for [pool_pages, page_rows, kv_heads, dim].  Pages that others hold are
- * the business of pages_reserve. */
+ * the business of pages_reserve; where *refused is not 0 (device, may be NULL: the
+ * book's word), nothing is written. */
 typedef struct tnsr_b200_paged_append_args {
     const void *k, *v;
     void *k_pool, *v_pool;
@@ -896,6 +902,7 @@ typedef struct tnsr_b200_paged_append_args {
     uint64_t k_page, k_row, k_head, v_page, v_row, v_head;
     uint32_t sequences, chunk, rows, k_ld, v_ld, kv_heads, dim, vdim, table_ld, page_rows, pool_pages;
     int32_t dtype;
+    const uint32_t* refused;
 } tnsr_b200_paged_append_args;
 TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args, void* stream);
 

@@ -109,7 +109,7 @@ class BeamSelectArgs(C.Structure):
 
 class PageBook(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("table", "lengths", "holders", "workspace", "d_status")] + [("workspace_bytes", C.c_uint64)] + \
-        [(n, C.c_uint32) for n in ("sequences", "table_ld", "page_rows", "pool_pages")]
+        [(n, C.c_uint32) for n in ("sequences", "table_ld", "page_rows", "pool_pages")] + [("refused", C.c_void_p)]
 
 
 class PagePools(C.Structure):
@@ -120,7 +120,7 @@ class PagedAppendArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_pool", "v_pool", "table", "lengths", "row_starts", "d_status")] + \
         [(n, C.c_uint64) for n in ("k_page", "k_row", "k_head", "v_page", "v_row", "v_head")] + \
         [(n, C.c_uint32) for n in ("sequences", "chunk", "rows", "k_ld", "v_ld", "kv_heads", "dim", "vdim", "table_ld", "page_rows", "pool_pages")] + \
-        [("dtype", C.c_int32)]
+        [("dtype", C.c_int32), ("refused", C.c_void_p)]
 
 
 class PagedAttentionArgs(C.Structure):

@@ -401,7 +401,7 @@ static const char* pools_problem(const tnsr_b200_page_pools* pools) {
     return nullptr;
 }
 static PageBook page_book(const tnsr_b200_page_book* b) {
-    return PageBook{b->table, b->lengths, b->holders, b->d_status, b->sequences, b->table_ld, b->page_rows, b->pool_pages, b->workspace};
+    return PageBook{b->table, b->lengths, b->holders, b->d_status, b->sequences, b->table_ld, b->page_rows, b->pool_pages, b->workspace, b->refused};
 }
 static PagePools page_pools(const tnsr_b200_page_pools* p) { return PagePools{p->tensors, p->page_bytes, p->count}; }
 static int bad_pages(const char* what, const char* problem) { return bad((std::string(what) + ": " + problem).c_str()); }
@@ -451,7 +451,7 @@ int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args, void* stream
     p.k = a.k; p.v = a.v; p.k_pool = a.k_pool; p.v_pool = a.v_pool; p.table = a.table; p.lengths = a.lengths; p.row_starts = a.row_starts;
     p.d_status = a.d_status; p.k_page = a.k_page; p.k_row = a.k_row; p.k_head = a.k_head; p.v_page = a.v_page; p.v_row = a.v_row; p.v_head = a.v_head;
     p.sequences = a.sequences; p.chunk = a.chunk; p.rows = a.rows; p.k_ld = a.k_ld; p.v_ld = a.v_ld; p.kv_heads = a.kv_heads; p.dim = a.dim;
-    p.vdim = a.vdim; p.table_ld = a.table_ld; p.page_rows = a.page_rows; p.pool_pages = a.pool_pages;
+    p.vdim = a.vdim; p.table_ld = a.table_ld; p.page_rows = a.page_rows; p.pool_pages = a.pool_pages; p.refused = a.refused;
     const OverlapLaunches overlap(as_stream(stream));
     return launch_paged_append(p, a.dtype, as_stream(stream));
 }

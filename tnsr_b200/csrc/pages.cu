@@ -324,8 +324,14 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
     }
     uint32_t all, all_copies;
     uint32_t at = block_scan(want, all), copy_at = block_scan(copies, all_copies);
+    // appended rows would go over old ones: whoever appends behind this call asks the word
+    auto outcome = [&](uint32_t what) {
+        if (threadIdx.x) return;
+        if (what) report(b.d_status, (int)what);
+        if (b.refused) *b.refused = what;
+    };
     if (bad) {
-        if (threadIdx.x == 0) report(b.d_status, bad);
+        outcome(bad);
         return;
     }
     for (uint32_t s = s0; s < s1; ++s) {
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
         copy_at += copy;
     }
     if (all > b.pool_pages || list_pages(b.holders, b.pool_pages, all, ws.pages, [](uint32_t h, uint32_t) { return h == 0; }) < all) {
-        if (threadIdx.x == 0) report(b.d_status, DEV_NO_PAGES);
+        outcome(DEV_NO_PAGES);
         return;
     }
     __syncthreads();
@@ -365,6 +371,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
     __syncthreads();
     for (uint32_t s = s0; s < s1; ++s) b.lengths[s] += rows ? rows[s] : rows_each;
     if (threadIdx.x == 0) ws.header[0] = all_copies;
+    outcome(0);
 }
 
 int launch_pages_reserve(const PageBook& b, const PagePools& pools, const uint32_t* rows, uint32_t rows_each, cudaStream_t stream) {
@@ -434,6 +441,7 @@ template <typename U>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedParams p, PagedAppend a, uint32_t k_units, uint32_t v_units, uint32_t per_unit) {
     pdl_wait();
     pdl_trigger();
+    if (a.refused && *a.refused) return;                         // no room for the rows: what lies at their places is older
     const uint32_t row = blockIdx.x;
     uint32_t s = row / a.chunk;
     if (a.row_starts) {           // the last sequence that starts at or before the row

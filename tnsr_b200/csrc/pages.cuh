@@ -10,6 +10,7 @@ struct PageBook {
     int* d_status;
     uint32_t sequences, table_ld, page_rows, pool_pages;
     void* workspace;
+    uint32_t* refused;              // what became of the last reserve, or null
 };
 struct PagePools {
     void* const* tensors;
@@ -34,6 +35,7 @@ struct PagedAppend {
     int* d_status;
     uint64_t k_page, k_row, k_head, v_page, v_row, v_head;
     uint32_t sequences, chunk, rows, k_ld, v_ld, kv_heads, dim, vdim, table_ld, page_rows, pool_pages;
+    const uint32_t* refused;
 };
 int launch_paged_append(const PagedAppend& a, int dtype, cudaStream_t stream);
 

@@ -1,6 +1,7 @@
 """Steps whose reserve is refused: what is appended behind it, queued or captured, leaves the caches as they are."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -8,7 +9,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from tests.gpu_util import _KEEP, lib, ok, ptr, stream  # noqa: E402
-from tests.paged_util import host, u32  # noqa: E402
+from tests.paged_util import host, scratch, status_word, u32  # noqa: E402
 from tests.test_gpu_h_beam_search import Book  # noqa: E402
 from tnsr_b200 import _native  # noqa: E402
 
@@ -98,3 +99,32 @@ def test_the_word_is_optional_and_follows_the_last_reserve():
     ok(lib().tnsr_b200_pages_reserve(C.byref(book.c_book), C.byref(book.c_pools), None, 1, stream()))
     torch.cuda.synchronize()
     assert host(word).tolist() == [4] and int(book.status[0]) == 4
+
+
+@pytest.mark.parametrize("sequences,rows,page_rows", [(12288, 349526, 1), (12288, 2 * 349526, 2)])
+def test_more_pages_are_wanted_than_32_bits_count(sequences, rows, page_rows):
+    """12288 x 349526 = 2^32 + 8192 pages of a pool of 10000: refused, and nothing has changed."""
+    ld, pool = -(-rows // page_rows), 10000
+    assert sequences * ld % (1 << 32) < pool
+    table = torch.empty(sequences * ld, dtype=torch.int32, device="cuda")
+    lengths, holders, status, word = u32(np.zeros(sequences)), u32(np.zeros(pool)), status_word(), u32([0])
+    work = scratch(lib().tnsr_b200_pages_workspace(sequences, pool))
+    book = _native.PageBook(table=table.data_ptr(), lengths=lengths.data_ptr(), holders=holders.data_ptr(), workspace=work.data_ptr(), d_status=status.data_ptr(),
+                            workspace_bytes=work.numel(), sequences=sequences, table_ld=ld, page_rows=page_rows, pool_pages=pool, refused=word.data_ptr())
+    pools = _native.PagePools(count=0)
+    ok(lib().tnsr_b200_pages_reserve(C.byref(book), C.byref(pools), None, rows, stream()))
+    torch.cuda.synchronize()
+    assert int(status[0]) == 5 and host(word).tolist() == [5]
+    assert int(lengths.abs().max()) == 0 and int(holders.abs().max()) == 0
+    # what there is room for is granted
+    status.zero_()
+    few = np.zeros(sequences)
+    few[[0, 5, sequences - 1]] = [4000 * page_rows, 1, 5999 * page_rows]
+    few_rows = u32(few)
+    ok(lib().tnsr_b200_pages_reserve(C.byref(book), C.byref(pools), few_rows.data_ptr(), 0, stream()))
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0 and int(holders.sum()) == 10000 and host(lengths).tolist() == few.astype(int).tolist()
+    rows_of = table.view(sequences, ld)
+    assert rows_of[0, :4000].tolist() == list(range(4000)) and rows_of[5, 0] == 4000 and rows_of[sequences - 1, :5999].tolist() == list(range(4001, 10000))
+    del table, rows_of
+    torch.cuda.empty_cache()

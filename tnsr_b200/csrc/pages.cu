@@ -272,10 +272,12 @@ __device__ uint32_t list_pages(const uint32_t* holders, uint32_t pool, uint32_t 
 
 __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, const uint32_t* rows, uint32_t rows_each, PageScratch ws) {
     __shared__ uint32_t s_bad;
+    __shared__ uint32_t s_many;                  // wanted pages in units of 8192, rounded down per thread
     pdl_wait();
     pdl_trigger();
     if (threadIdx.x == 0) {
         s_bad = 0;
+        s_many = 0;
         ws.header[0] = 0;
     }
     __syncthreads();
@@ -310,7 +312,8 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
     }
     __syncthreads();
     const uint32_t bad = s_bad;
-    uint32_t want = 0, copies = 0;
+    uint64_t want = 0;
+    uint32_t copies = 0;
     for (uint32_t s = s0; s < s1; ++s) {
         const uint32_t page = ws.source[s];
         if (page != PG_NONE && __ldcg(ws.writers + page) == b.holders[page] && __ldcg(ws.keeper + page) == ~s) ws.source[s] = PG_NONE;   // keeps it
@@ -322,8 +325,11 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
         want += pages_of(length + n, b.page_rows) - pages_of(length, b.page_rows) + copy;
         copies += copy;
     }
+    // Twelve sequences of 2^31 pages a thread at the most.  Above 2^18 units there are more than a pool's 2^30 pages; else there are fewer than 2^32 in all, and the sums
+    // below are exact.
+    if (want >> 13) atomicAdd(&s_many, (uint32_t)(want >> 13));
     uint32_t all, all_copies;
-    uint32_t at = block_scan(want, all), copy_at = block_scan(copies, all_copies);
+    uint32_t at = block_scan((uint32_t)want, all), copy_at = block_scan(copies, all_copies);      // with barriers
     // appended rows would go over old ones: whoever appends behind this call asks the word
     auto outcome = [&](uint32_t what) {
         if (threadIdx.x) return;
@@ -342,7 +348,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(PageBook b, c
         at += pages_of(length + n, b.page_rows) - pages_of(length, b.page_rows) + copy;
         copy_at += copy;
     }
-    if (all > b.pool_pages || list_pages(b.holders, b.pool_pages, all, ws.pages, [](uint32_t h, uint32_t) { return h == 0; }) < all) {
+    if (s_many > 1u << 18 || all > b.pool_pages || list_pages(b.holders, b.pool_pages, all, ws.pages, [](uint32_t h, uint32_t) { return h == 0; }) < all) {
         outcome(DEV_NO_PAGES);
         return;
     }

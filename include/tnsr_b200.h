@@ -782,7 +782,8 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
  * All of it is device work on the caller's stream, without synchronisation.  The
  * entry points below share these rules.
  *  - A status word (`d_status`, a device int that the caller clears, may be NULL)
- *    keeps the first problem that a kernel meets: 3 = a sequence has more rows than
+ *    keeps the first problem that a kernel meets: 2 = a bounded wait gave up
+ *    (tnsr_b200_set_wait_limit_ns), and the call's outputs are not to be used; 3 = a sequence has more rows than
  *    its table row can name, or fewer than a call brings or needs; 4 = a table
  *    entry that a call follows names no page of the pool; 5 = more pages wanted than
  *    are free; 6 = a parent outside its group.  Nothing outside the given tables,
@@ -822,6 +823,7 @@ typedef struct tnsr_b200_beam_select_args {
     uint64_t workspace_bytes, logits_ld;
     uint32_t groups, beams, vocab, keep, end_token;
     int32_t dtype;
+    int* d_status;                /* may be NULL; 2: a bounded wait gave up, and beams count as such without a sum */
 } tnsr_b200_beam_select_args;
 /* Enough for calls of fewer groups, beams, tokens and candidates too. */
 TNSR_B200_API uint64_t tnsr_b200_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t keep);
@@ -918,7 +920,7 @@ TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args
  * head h / (heads / kv_heads).  dim, vdim <= 256.  Scores, maxima, sums and
  * accumulators are f32; with dtype bf16 the weights of a value product keep 16
  * bits for few rows, 8 bits for many.  Keys in a page outside the pool (status 4)
- * count as zeros.  Status 2: a bounded wait inside the kernel for many rows gave up.
+ * count as zeros.
  * workspace: tnsr_b200_paged_attention_workspace() bytes; NULL: the keys of a
  * sequence are not divided.  The same call gives the same bits; where the keys of a
  * sequence are divided, and with it the last bits of its sums, depends on the

@@ -104,7 +104,7 @@ class Mamba2Args(C.Structure):
 class BeamSelectArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("logits", "scores", "finished", "next_scores", "tokens", "parents", "next_finished", "workspace")] + \
         [(n, C.c_uint64) for n in ("workspace_bytes", "logits_ld")] + \
-        [(n, C.c_uint32) for n in ("groups", "beams", "vocab", "keep", "end_token")] + [("dtype", C.c_int32)]
+        [(n, C.c_uint32) for n in ("groups", "beams", "vocab", "keep", "end_token")] + [("dtype", C.c_int32), ("d_status", C.c_void_p)]
 
 
 class PageBook(C.Structure):

@@ -15,6 +15,7 @@ struct BeamSelect {
     void* workspace;
     uint64_t workspace_bytes, logits_ld;
     uint32_t groups, beams, vocab, keep, end_token;
+    int* d_status;                 // or null
 };
 constexpr uint32_t BEAM_MAX = 32, BEAM_MAX_KEEP = 64;
 constexpr uint32_t BEAM_MAX_VOCAB = 1u << 26;

@@ -19,6 +19,7 @@
 #include <cmath>
 
 #include "beam.cuh"
+#include "paged.cuh"
 #include "tc_common.cuh"
 
 namespace tb {
@@ -369,7 +370,10 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_scan_kernel(BeamSelect b, 
     double sum = 0.0;
     for (uint32_t i = 0; i < pieces; ++i) {
         const uint32_t stage = i % BS_STAGES, base = first + i * BS_PIECE, here = min(end - base, BS_PIECE);
-        if (!mbar_wait(full + stage, (i / BS_STAGES) & 1, &gave_up, wait_limit_ns)) sum = nan("");      // the row does not count then
+        if (!mbar_wait(full + stage, (i / BS_STAGES) & 1, &gave_up, wait_limit_ns)) {                    // the row does not count then
+            sum = nan("");
+            report(b.d_status, DEV_TIMEOUT);
+        }
         // value j * W + e of the thread is number (j * BS_THREADS + tid) * W + e of the piece; what is not there is -inf
         float v[16];
         const uint8_t* src = space + stage * BeamStage<T>::BYTES + skew;

@@ -370,6 +370,7 @@ int tnsr_b200_beam_select(const tnsr_b200_beam_select_args* args, void* stream) 
     b.logits = args->logits; b.scores = args->scores; b.finished = args->finished; b.next_scores = args->next_scores; b.tokens = args->tokens;
     b.parents = args->parents; b.next_finished = args->next_finished; b.workspace = args->workspace; b.workspace_bytes = args->workspace_bytes;
     b.logits_ld = args->logits_ld; b.groups = args->groups; b.beams = args->beams; b.vocab = args->vocab; b.keep = args->keep; b.end_token = args->end_token;
+    b.d_status = args->d_status;
     const OverlapLaunches overlap(as_stream(stream));
     return launch_beam_select(b, args->dtype, as_stream(stream));
 }

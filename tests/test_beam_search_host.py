@@ -141,3 +141,9 @@ def test_a_selections_workspace_is_enough_for_smaller_ones(library):
             assert sizes == sorted(sizes)
     for big, small in (((40, 8, 50000, 16), (39, 3, 50000, 16)), ((40, 8, 50000, 16), (40, 8, 2048, 16)), ((40, 8, 50000, 16), (1, 1, 49999, 1))):
         assert need(*big) >= need(*small)
+
+
+def test_more_rows_and_heads_than_a_grid_has_room_for_are_refused(library):
+    for rows, heads, dim in ((1 << 30, 8, 1), (0x7fffffff, 5, 1), (1 << 25, 260, 7)):
+        refuses(library.tnsr_b200_paged_attention(C.byref(attend(rows=rows, sequences=rows, heads=heads, kv_heads=1, dim=dim, vdim=dim, q_ld=heads * dim, out_ld=heads * dim)),
+                                                  None), "too many rows")

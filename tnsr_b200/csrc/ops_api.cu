@@ -465,6 +465,7 @@ int tnsr_b200_paged_attention(const tnsr_b200_paged_attention_args* args, void* 
     if (!a.q || !a.out) return bad("paged_attention: null pointer");
     if (a.heads == 0 || a.heads > 0x7fffffffu || a.heads % a.kv_heads || a.q_ld < (uint64_t)a.heads * a.dim || a.out_ld < (uint64_t)a.heads * a.vdim)
         return bad("paged_attention: kv_heads must divide heads, and rows must hold every head");
+    if ((uint64_t)a.rows * a.heads > 4 * 0x7fffffffull) return bad("paged_attention: too many rows and heads");       // four of them to a block of a grid
     if (a.dim > 256 || a.vdim > 256) {
         set_thread_error("paged_attention: widths are at most 256");
         return TNSR_B200_ERR_UNSUPPORTED;

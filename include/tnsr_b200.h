@@ -840,7 +840,8 @@ TNSR_B200_API int tnsr_b200_reorder_states(void* const* tensors, const uint64_t*
 
 /* Who holds which page of a pool.  table [sequences, table_ld]: the pages of a
  * sequence in order, the first ceil(lengths / page_rows) entries of a row live, the
- * others never read.  holders [pool_pages]: live entries that name the page, 0 for a
+ * others never read (a length of more rows than the entries name counts as all of
+ * them, status 3).  holders [pool_pages]: live entries that name the page, 0 for a
  * free one.  An empty book is lengths and holders of zero.  sequences <= 12288. */
 typedef struct tnsr_b200_page_book {
     uint32_t *table, *lengths, *holders;

@@ -46,8 +46,12 @@ static PageScratch page_scratch(void* ws, uint32_t sequences, uint32_t pool_page
 uint64_t pages_workspace_bytes(uint32_t sequences, uint32_t pool_pages) { return 4ull * (16 + 5ull * pool_pages + 3ull * sequences + 1); }
 
 static __device__ __forceinline__ uint32_t pages_of(uint32_t rows, uint32_t page_rows) { return rows / page_rows + (rows % page_rows != 0); }
-// Pages of sequence s; more than its table row has room for is the caller's mistake.
-static __device__ __forceinline__ uint32_t live_pages(const PageBook& b, uint32_t s) { return min(pages_of(b.lengths[s], b.page_rows), b.table_ld); }
+// Pages of sequence s; more than its table row has room for is the caller's mistake, and told.
+static __device__ __forceinline__ uint32_t live_pages(const PageBook& b, uint32_t s) {
+    const uint32_t n = pages_of(b.lengths[s], b.page_rows);
+    if (n > b.table_ld) report(b.d_status, DEV_BAD_LENGTH);
+    return min(n, b.table_ld);
+}
 
 // Exclusive prefix sum over the block in thread order, and the total.
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t& total) {
@@ -85,6 +89,7 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(PageBook b, const uint3
     const uint32_t column0 = blockIdx.x * columns, here = min(columns, b.table_ld - column0), cells = b.sequences * here;
     for (uint32_t s = threadIdx.x; s < b.sequences; s += blockDim.x) {
         lengths[s] = b.lengths[s];
+        if (blockIdx.x == 0 && pages_of(lengths[s], b.page_rows) > b.table_ld) report(b.d_status, DEV_BAD_LENGTH);
         uint32_t p = parents[s];
         if (p >= b.sequences) {
             if (blockIdx.x == 0) report(b.d_status, DEV_BAD_PARENT);

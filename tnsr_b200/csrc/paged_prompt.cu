@@ -553,8 +553,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // the list was that of the item before the last one
             if (number >= 2 && !wait(read + slot, ((number >> 1) - 1) & 1)) break;
             uint32_t count = 0;
+            bool sees[2] = {false, false};
             for (uint32_t j = j0; j < j1; ++j, ++blocks) {
                 const uint32_t stage = blocks % STAGES, key0 = item_key0(it, j);
+                sees[0] |= tile_sees(p, it, 0, key0);
+                sees[1] |= tile_sees(p, it, 1, key0);
                 ok = wait(v_full + stage, (blocks / STAGES) & 1);
                 if (!ok) break;
                 if (partly_seen(p, it, 0, it.tokens[1] ? 1 : 0, key0)) {
@@ -593,7 +596,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (!ok) break;
             if (lane == 0) odd_count[slot] = count;
             __syncwarp();
-            if (lane == 0) mbar_arrive(listed + slot);
+            if (lane == 0) {
+                mbar_arrive(listed + slot);
+                // for the warps of a tile that sees nothing here, which pass the item over
+                for (int n = (sees[0] ? 0 : 4) + (sees[1] ? 0 : 4); n > 0; --n) mbar_arrive(read + slot);
+            }
             ++number;
         }
     }
@@ -614,7 +621,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         while (ok && walk.more(prm, plan)) {
             if (!walk.step(prm, plan, it)) continue;
             const uint32_t j0 = walk.begin(), j1 = walk.end(it);
-            // the item's list, once it is complete: which keys' values must not be multiplied by 0 (`mine`, the row sees one of them).  Every warp takes every list.
+            if (!it.tokens[t]) {
+                if (it.blocks) ++number;
+                continue;
+            }
+            // Whether the row (`mine`) sees a key whose values must not be multiplied by 0: by the item's list, once it is complete.  For warps that have waited for
+            // products of this item, so that no earlier turn of the barrier is taken for this one.
             auto odd_in_sight = [&](bool mine, int32_t at) {
                 const uint32_t slot = number & 1;
                 if (!wait(listed + slot, (number >> 1) & 1)) ok = false;
@@ -627,13 +639,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(read + slot);
-                ++number;
                 return odd && mine;
             };
-            if (!it.tokens[t]) {
-                if (it.blocks) odd_in_sight(false, 0);
-                continue;
-            }
             const int32_t at = it.first[t] + (int32_t)min(my_token, it.tokens[t] - 1);
             const int32_t lowest = p.a.window ? at - (int32_t)min(p.a.window, 0x7fffffffu) + 1 : 0;
             float m = -INFINITY, l = 0.0f;
@@ -723,8 +730,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ++outputs;
                 tc_fence_after();
             }
-            bool mine = my_token < it.tokens[t], odd = it.blocks && odd_in_sight(mine, at);
+            bool mine = my_token < it.tokens[t], odd = any && odd_in_sight(mine, at);
             if (!ok) break;
+            if (it.blocks) ++number;
             mine &= !odd;
             bf16* out = reinterpret_cast<bf16*>(p.a.out) + (uint64_t)(it.seq.start + it.token0 + t * prm.tokens + my_token) * p.a.out_ld +
                         (uint64_t)(it.kvh * p.per.d + my_head) * p.a.vdim;

@@ -891,7 +891,8 @@ TNSR_B200_API int tnsr_b200_pages_copy(const tnsr_b200_page_pools* pools, const 
  * row_starts[s] .. row_starts[s + 1] (device [sequences + 1], in order, at most
  * `chunk` each) or, with row_starts NULL, `chunk` rows each; they are the last rows
  * of its lengths[s].  rows: how many the arrays hold; rows of no sequence are left
- * out.  k [rows, kv_heads, dim] with k_ld elements between rows, v likewise with
+ * out, and so are those of one that brings more than `chunk` or is longer than its
+ * table row can name (status 3).  k [rows, kv_heads, dim] with k_ld elements between rows, v likewise with
  * vdim: slices of a fused projection will do.  Element (page, row, head, i) of a
  * pool lies at page * k_page + row * k_row + head * k_head + i, in elements; three
  * zeros stand for [pool_pages, page_rows, kv_heads, dim].  Pages that others hold are

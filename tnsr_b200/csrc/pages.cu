@@ -466,6 +466,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedParams p, PagedA
     const PagedSequence q = paged_sequence(p, s);
     const uint32_t i = row - q.start;
     if (row < q.start || i >= q.count) return;                  // behind the last sequence
+    // cut lengths and counts (told by now) would put rows where others are
+    if (a.lengths[s] > p.capacity || (a.row_starts && min(a.row_starts[s + 1], a.rows) - q.start > a.chunk)) return;
     if (q.length < q.count - i) {                               // the cache has no such row
         if (threadIdx.x == 0) report(a.d_status, DEV_BAD_LENGTH);
         return;

@@ -789,7 +789,7 @@ TNSR_B200_API int tnsr_b200_argmax(const float* logits, uint32_t* out, uint32_t 
  *    are free; 6 = a parent outside its group.  Nothing outside the given tables,
  *    pools and rows is read or written in such a case.
  *  - A workspace is device memory, 16-byte aligned, zeroed once before its first
- *    use (again if a launch was cut short by a device error); calls leave it ready
+ *    use (again behind status 2, or a launch that a device error cut short); calls leave it ready
  *    for the next one, of the same operator (fork, reserve and compact: of any of
  *    them, on any book) at any sizes that it is large enough for.
  *    Calls that may overlap on the GPU must not share one, and two captured graphs
@@ -921,7 +921,12 @@ TNSR_B200_API int tnsr_b200_paged_append(const tnsr_b200_paged_append_args* args
  * [rows, heads, vdim] with out_ld elements between rows; head h reads key/value
  * head h / (heads / kv_heads).  dim, vdim <= 256.  Scores, maxima, sums and
  * accumulators are f32; with dtype bf16 the weights of a value product keep 16
- * bits for few rows, 8 bits for many.  Keys in a page outside the pool (status 4)
+ * bits or more for few rows, 8 bits for many.  Few are chunk * heads / kv_heads <= 16, and
+ * up to 64 while the units of 16 of them (of all sequences and key/value heads) are
+ * no more than 148; and all rows of widths above 128, of strides or addresses that
+ * are no multiples of 16 bytes, of pages whose rows are no multiple of 8, or with
+ * scale <= 0.  The bound `chunk` decides, not the rows that a sequence brings: it is
+ * best the largest number of them (and prompts and single tokens two calls).  Keys in a page outside the pool (status 4)
  * count as zeros.
  * workspace: tnsr_b200_paged_attention_workspace() bytes; NULL: the keys of a
  * sequence are not divided.  The same call gives the same bits; where the keys of a

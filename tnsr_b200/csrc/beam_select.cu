@@ -13,8 +13,8 @@
 // of a group's joins its runs in the same way.
 //
 // Sums: 16 terms in f32, the rest in f64.  A block's order of terms does not depend on the row, so that equal rows have equal sums to the last bit.
-// Bound by HBM (each logit once) for large groups, else by the chain of barriers behind the reading: 48 groups x 6 beams x 50021 logits, keep 12, 22.6 us =
-// 2.55 TB/s (one wave of blocks: reading is half of it); one group x 4 beams x 32000, keep 4, 9.8 us.
+// Bound by HBM (each logit once) for large groups, else by the chain of barriers behind the reading: 48 groups x 6 beams x 50021 logits, keep 12, 22.8 us =
+// 2.53 TB/s (one wave of blocks: reading is half of it); one group x 4 beams x 32000, keep 4, 9.8 us.
 #include <algorithm>
 #include <cmath>
 

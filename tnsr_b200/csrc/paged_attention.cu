@@ -840,7 +840,8 @@ __global__ void __launch_bounds__(160, W == 64 ? 3 : W == 128 ? 2 : 1) paged_few
 namespace {
 // Rows (tokens x heads of a group) of a sequence up to which this kernel takes bf16 calls that the other one for many rows could take: a unit of 16 always, up to 64
 // while all units find an SM each, for every unit reads the keys for itself.  us here / there, heads of 128, 4 per key/value head: one sequence of 4096 keys, 32 / 64 /
-// 256 rows 19 / 32, 24 / 32, 50 / 38; 16 of 2048, 32 / 64 rows 42 / 39, 69 / 39; 64 of 1024, 64 rows 150 / 70.
+// 256 rows 19 / 31, 24 / 31, 50 / 37; 16 of 2048, 32 / 64 rows 42 / 38, 69 / 38; 64 of 1024, 64 rows 150 / 71.
+// Rows are known by their bound, `chunk`: what a sequence brings stands on the device.
 constexpr uint32_t FEW_ROWS = 64, FEW_UNITS = 148;
 
 uint32_t few_width(uint32_t dim, uint32_t vdim) {
@@ -903,7 +904,7 @@ uint64_t paged_attention_workspace_bytes(uint32_t dim, uint32_t vdim, int dtype)
 int launch_paged_attention(const PagedAttention& args, int dtype, cudaStream_t stream) {
     if (args.rows == 0 || args.sequences == 0) return TNSR_B200_OK;
     PagedAttention a = args;
-    a.chunk = std::min(a.chunk, a.rows);             // no sequence has more: a generous bound costs nothing
+    a.chunk = std::min(a.chunk, a.rows);             // no sequence has more
     PagedParams p;
     p.a = a;
     p.page = fast_div(a.page_rows);

@@ -28,7 +28,7 @@
 // Every wait is bounded as elsewhere: one that gives up raises the abort flag, the roles fall through and the status word is set.
 //
 // Bound by a tile's chain of scores, softmax and product: 4050 cycles for a pair of blocks, of which the special functions need 2050 and the products 2660.  6000 rows
-// over 12000 keys, window 4096, 32 / 8 heads of 128 (404 GFLOP): 461 us = 877 TFLOP/s.
+// over 12000 keys, window 4096, 32 / 8 heads of 128 (404 GFLOP): 448 us = 902 TFLOP/s (485 among other work).
 #include <algorithm>
 
 #include "mixers.cuh"
@@ -889,7 +889,7 @@ int launch_paged_prompt(const PagedParams& p, cudaStream_t stream) {
     prm.box = std::min(128u, a.page_rows & (0u - a.page_rows));
     prm.wait_limit_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
     // The last round is divided where it can pay: items of more key blocks than the joins cost, and (as far as can be told here) a round that leaves a quarter of
-    // the grid idle.  One prompt of 6000 rows over 12000 keys, window 4096, 32 / 8 heads: 487 -> 460 us; 3 x 100 rows over up to 4000 keys: 74 -> 47; where nothing
+    // the grid idle.  One prompt of 6000 rows over 12000 keys, window 4096, 32 / 8 heads: 472 -> 447 us; 3 x 100 rows over up to 4000 keys: 70 -> 47; where nothing
     // pays the plan alone costs 2 to 4 us.
     const uint64_t entries = (uint64_t)a.sequences * prm.pairs;
     const uint32_t span = a.window ? (uint32_t)std::min<uint64_t>(p.capacity, (uint64_t)a.window + 2 * prm.tokens + std::min(a.sinks, p.capacity) + 256) : p.capacity;

@@ -12,8 +12,8 @@
 // The bookkeeping is integers: counters by atomics (sums do not depend on their order), choices by ranks (prefix sums in order of sequences and
 // pages), so a call's result is a function of its inputs.  What has an order runs in one block: 16 sequences x 4 beams with 40 entries each take
 // a few us, which is the latency of a chain of dependent reads, and the search for free pages ends at the last one that is needed.
-// What bounds a call that copies is the copying: 16-byte loads, eight on their way per thread (compaction of 512 MB: 117 us, 4.6 TB/s read and written; 4 or 16
-// blocks an SM are level with 8).  Fork and reserve of 64 sequences with 24 pools: 18.5 us, three launches that wait for one another.
+// What bounds a call that copies is the copying: 16-byte loads, eight on their way per thread (compaction of 512 MB: 117 us, of which the copying takes 102, 5.3 TB/s read and written, and
+// the plan before it the rest; 4 or 16 blocks an SM are level with 8).  Fork and reserve of 64 sequences with 24 pools: 18.5 us, three launches that wait for one another.
 //
 // Also here: rows appended to caches in pages, and states reordered to their sequences' parents.
 #include <algorithm>
@@ -519,7 +519,7 @@ int launch_paged_append(const PagedAppend& a, int dtype, cudaStream_t stream) {
 
 // ---- states to their sequences' parents -------------------------------------------------------------------------------------------
 // A thread has the same unit of every row of a group: it reads what moves, then writes, so the rows trade places without a copy of them
-// and without waiting for anybody.  Rows that stay are neither read nor written.  Bound by HBM: 247 MB moved, 47 us = 5.2 TB/s.
+// and without waiting for anybody.  Rows that stay are neither read nor written.  Bound by HBM: 247 MB moved, 46 to 50 us = 4.9 to 5.4 TB/s.
 constexpr uint32_t RO_TENSORS = 64;
 struct StateList {
     uint8_t* at[RO_TENSORS];
